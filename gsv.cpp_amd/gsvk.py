@@ -32,7 +32,8 @@ EXPORTS = [
     "gsvk_op_attn_decode_noalloc", "gsvk_model_set_decode_path", "gsvk_op_dec_attn", "gsvk_op_dec_ffn",
     "gsvk_model_set_exact", "gsvk_op_attn_exact", "gsvk_op_expf_exact", "gsvk_model_set_prefill_f16",
     "gsvk_op_q8_dequant_f16", "gsvk_op_q8h_gemm", "gsvk_op_qkv_attn_exact", "gsvk_model_get_profile",
-    "gsvk_model_time_decode_kernel", "gsvk_phase_stamps",
+    "gsvk_model_time_decode_kernel", "gsvk_phase_stamps", "gsvk_op_paged_append", "gsvk_op_attn_paged",
+    "gsvk_attn_paged_workspace_bytes",
 ]
 
 GSVK_DECODE_AUTO, GSVK_DECODE_GEMV, GSVK_DECODE_FUSED, GSVK_DECODE_MFMA, GSVK_DECODE_PERSIST = 0, 1, 2, 3, 4
@@ -73,6 +74,23 @@ class ModelInfo(C.Structure):
                 ("ffn_dim", C.c_int), ("head_type", C.c_int), ("text_alpha", C.c_float),
                 ("audio_alpha", C.c_float), ("prompt_len", C.c_int), ("kv_batch", C.c_int),
                 ("kv_lmax", C.c_int)]
+
+
+GSVK_TYPE_F32, GSVK_TYPE_F16, GSVK_TYPE_BF16 = 0, 1, 30
+
+
+class PagedKVArgs(C.Structure):
+    """gsvk_paged_kv (include/gsvk.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int),
+                ("page_size", C.c_int), ("n_pages", C.c_int64), ("page_stride", C.c_int64), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_cols", C.c_int), ("B", C.c_int), ("seq_start", C.c_void_p),
+                ("kv_len", C.c_void_p)]
+
+
+class RopeArgs(C.Structure):
+    """gsvk_rope (include/gsvk.h)."""
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("rows", C.c_int64), ("rot", C.c_int), ("pairs", C.c_int),
+                ("pos", C.c_void_p)]
 
 
 class BertInfo(C.Structure):
@@ -151,6 +169,12 @@ def lib():
         L.gsvk_sample_workspace_bytes.argtypes = [i32]
         L.gsvk_sample_workspace_bytes.restype = C.c_size_t
         L.gsvk_op_sample.argtypes = [vp, i32, i32, vp, i32, vp, C.POINTER(SamplerCfg), vp, vp, vp, vp, vp]
+        L.gsvk_op_paged_append.argtypes = [C.POINTER(PagedKVArgs), vp, vp, vp, i32, i64, i32, i64, i64, i64,
+                                           C.POINTER(RopeArgs), vp, vp, vp]
+        L.gsvk_attn_paged_workspace_bytes.argtypes = [C.POINTER(PagedKVArgs), i64, i32, i32, i64]
+        L.gsvk_attn_paged_workspace_bytes.restype = C.c_size_t
+        L.gsvk_op_attn_paged.argtypes = [C.POINTER(PagedKVArgs), vp, i64, i32, i64, i32, i64, f32, i32, vp, vp, i32,
+                                         i64, vp, vp, C.c_size_t, vp]
         _lib = L
     return _lib
 
@@ -327,6 +351,139 @@ def op_qkv_attn(wq, wd, bias, res, r, ln_bias, wb, k, v, kv_begin, col, scale, o
     fn = lib().gsvk_op_qkv_attn_exact if exact else lib().gsvk_op_qkv_attn
     check(fn(_p(wq), _p(wd), _p(bias), _p(res), _p(r), _p(ln_bias), _p(wb), B, nh, _p(k), _p(v), lstride,
              _p(kv_begin), _p(col), scale, _p(out), _p(oq), _p(od), _p(ln_out), _stream(stream)), "qkv_attn")
+
+
+def _gsvk_type(dtype):
+    """GGML type number of a torch dtype (F32, F16 or BF16)."""
+    name = str(dtype)
+    try:
+        return {"torch.float32": GSVK_TYPE_F32, "torch.float16": GSVK_TYPE_F16, "torch.bfloat16": GSVK_TYPE_BF16}[name]
+    except KeyError:
+        raise ValueError(f"gsvk: {name} is not a type of the paged-cache operators") from None
+
+
+def _rows_of(t, what, width, device):
+    """Row stride of a token array [T][width] or [T][heads][hd] whose rows are contiguous."""
+    inner = 1
+    for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if n != 1 and st != inner:
+            raise ValueError(f"{what}: the rows must be contiguous")
+        inner *= n
+    if t.dim() < 2 or inner != width:
+        raise ValueError(f"{what}: rows of {width} elements expected")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, the cache on {device}")
+    return t.stride(0) if t.shape[0] > 1 else inner
+
+
+def _int32(t, what, shape, device):
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what}: a contiguous int32 tensor of shape {list(shape)} on {device} expected")
+    return t
+
+
+class PagedKV:
+    """A cache in pages and the batch of a step (include/gsvk.h gsvk_paged_kv), kept by a program with
+    its buffers: k, v [n_pages][n_kv][page_size][hd] (pages may lie apart: any stride of dimension
+    0), table [B][cols] int32 (rows may lie apart), seq_start [B + 1] and kv_len [B] int32. The
+    operators read the tensors' contents when they run."""
+
+    def __init__(self, k, v, table, seq_start, kv_len):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("PagedKV: k and v must be [n_pages][n_kv][page_size][hd] alike")
+        n_pages, n_kv, page, hd = k.shape
+        inner = (page * hd, hd, 1)
+        if any(n != 1 and st != want for n, st, want in zip(k.shape[1:], k.stride()[1:], inner)):
+            raise ValueError("PagedKV: a page must be contiguous")
+        if not k.is_cuda or any(t.device != k.device for t in (v, table, seq_start, kv_len)):
+            raise ValueError("PagedKV: every tensor must be on the cache's device")
+        if table.dim() != 2 or str(table.dtype) != "torch.int32" or (table.shape[1] != 1 and table.stride(1) != 1):
+            raise ValueError("PagedKV: table must be [B][cols] int32 with contiguous rows")
+        B, cols = table.shape
+        _int32(seq_start, "PagedKV: seq_start", (B + 1,), k.device)
+        _int32(kv_len, "PagedKV: kv_len", (B,), k.device)
+        self.dtype, self.device, self.type = k.dtype, k.device, _gsvk_type(k.dtype)
+        self.n_kv, self.page_size, self.hd, self.B, self.cols = n_kv, page, hd, B, cols
+        self.keep = (k, v, table, seq_start, kv_len)
+        self.args = PagedKVArgs(k.data_ptr(), v.data_ptr(), self.type, n_kv, hd, page, n_pages,
+                                k.stride(0) if n_pages > 1 else 0, table.data_ptr(),
+                                table.stride(0) if B > 1 else cols, cols, B, seq_start.data_ptr(), kv_len.data_ptr())
+        self._ref = C.byref(self.args)
+
+    def _on_device(self, what):
+        import torch
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"{what}: the cache is on {self.device}, which is not the current device")
+
+
+def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=False, pos=None, n_bad=None,
+                    stream=None):
+    """Append k, v [T][n_kv * hd] to the pages of `kv` (PagedKV) and rotate q [T][nh * hd] into q_out
+    [T][nh][hd] (include/gsvk.h gsvk_op_paged_append); cos, sin [positions][rot / 2] fp32."""
+    kv._on_device("paged_append")
+    T, w = k.shape[0], kv.n_kv * kv.hd
+    if v.shape[0] != T or k.dtype != v.dtype or (q is None) != (q_out is None):
+        raise ValueError("paged_append: k and v of the same rows and type, q and q_out together")
+    ks, vs = _rows_of(k, "paged_append: k", w, kv.device), _rows_of(v, "paged_append: v", w, kv.device)
+    nh = qs = 0
+    if q is not None:
+        if q_out.dim() != 3 or q_out.shape[0] != T or q_out.shape[2] != kv.hd or not q_out.is_contiguous() \
+                or q_out.dtype != kv.dtype or q_out.device != kv.device or q.shape[0] != T or q.dtype != k.dtype:
+            raise ValueError("paged_append: q_out must be a dense [T][nh][hd] of the cache's type, q of k's type")
+        nh = q_out.shape[1]
+        qs = _rows_of(q, "paged_append: q", nh * kv.hd, kv.device)
+    rope = None
+    if cos is not None:
+        if sin is None or cos.dim() != 2 or cos.shape != sin.shape or not cos.is_contiguous() \
+                or not sin.is_contiguous() or str(cos.dtype) != "torch.float32" or cos.dtype != sin.dtype \
+                or cos.device != kv.device or sin.device != kv.device:
+            raise ValueError("paged_append: cos and sin must be [positions][rot / 2] fp32 alike")
+        if pos is not None:
+            _int32(pos, "paged_append: pos", (T,), kv.device)
+        rope = RopeArgs(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], 1 if pairs else 0,
+                        None if pos is None else pos.data_ptr())
+    elif sin is not None or pos is not None:
+        raise ValueError("paged_append: sin and pos go with cos")
+    if n_bad is not None:
+        _int32(n_bad, "paged_append: n_bad", (1,), kv.device)
+    check(lib().gsvk_op_paged_append(kv._ref, _p(q), _p(k), _p(v), _gsvk_type(k.dtype), T, nh, qs, ks, vs,
+                                     None if rope is None else C.byref(rope), _p(q_out), _p(n_bad),
+                                     _stream(stream)), "paged_append")
+
+
+def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys) -> int:
+    return int(lib().gsvk_attn_paged_workspace_bytes(kv._ref, tokens, nh, max_new, max_keys))
+
+
+def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0, prefix=None, ws=None, stream=None):
+    """Attention of the new tokens q [T][nh][hd] over the pages of `kv` (PagedKV) into out [T][nh][hd]
+    (include/gsvk.h gsvk_op_attn_paged); lse [T][nh] fp32, prefix [B] int32. ws None: a workspace from
+    torch's allocator, which belongs to torch's current stream."""
+    kv._on_device("attn_paged")
+    T, nh = q.shape[0], q.shape[1]
+    if q.dim() != 3 or out.shape != q.shape or q.dtype != kv.dtype:
+        raise ValueError("attn_paged: q of the cache's type and out must be [T][nh][hd]")
+    w = nh * kv.hd
+    qs, os_ = _rows_of(q, "attn_paged: q", w, kv.device), _rows_of(out, "attn_paged: out", w, kv.device)
+    if lse is not None and (tuple(lse.shape) != (T, nh) or str(lse.dtype) != "torch.float32"
+                            or not lse.is_contiguous() or lse.device != kv.device):
+        raise ValueError("attn_paged: lse must be a dense [T][nh] fp32")
+    if prefix is not None:
+        _int32(prefix, "attn_paged: prefix", (kv.B,), kv.device)
+    if max_keys is None:
+        max_keys = kv.cols * kv.page_size
+    if ws is None:
+        n = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys)
+        if n:
+            import torch
+            if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
+                raise ValueError("attn_paged: a stream other than torch's current one needs a ws of its own")
+            ws = torch.empty(n, dtype=torch.uint8, device=kv.device)
+    elif ws.device != kv.device or not ws.is_contiguous():
+        raise ValueError("attn_paged: ws must be a dense tensor on the cache's device")
+    check(lib().gsvk_op_attn_paged(kv._ref, _p(q), T, nh, qs, max_new, max_keys, scale, window, _p(prefix), _p(out),
+                                   _gsvk_type(out.dtype), os_, _p(lse), _p(ws),
+                                   0 if ws is None else ws.numel() * ws.element_size(), _stream(stream)), "attn_paged")
 
 
 def op_sample(logits, cfg, rng, tok_out, hist=None, n_hist=None, probs_out=None, ws=None, stream=None):

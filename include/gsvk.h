@@ -495,6 +495,102 @@ int gsvk_op_attn_prefill(const float * qkv, int B, int S, int max_len, const int
                          int hd, float scale, int path, float * out, int8_t * oq, float * od,
                          void * stream);
 
+/* ---- A cache in pages (paged K/V): sequences of any length share one cache -----------------
+ * The cache is n_pages pages; the page table of a sequence names the pages that hold its keys in
+ * order, so requests join, grow and leave without a cache being moved or padded. No counterpart in
+ * the reference (its cache is [n_layer][B][n_head][lmax + 1][hd], src/gsv_ar.cpp:94-118). The two
+ * operators below serve every form of a step: one new token per sequence, chunks of prompts, a few
+ * drafted tokens, or a mix. They allocate nothing, never synchronise and can be captured into a
+ * graph; every array below is device memory that they read at run time, so a captured graph
+ * follows what the arrays hold when it is replayed. */
+
+/* element types, by their GGML numbers */
+#define GSVK_TYPE_F32  0
+#define GSVK_TYPE_F16  1
+#define GSVK_TYPE_BF16 30
+
+/* A paged cache and the batch of sequences that a step works on.
+ *  k, v        : pages of [n_kv][page_size][hd] elements of `type` (GSVK_TYPE_F16 or _BF16),
+ *                page_stride elements from one page to the next (0 = dense; larger where a page
+ *                holds several layers, or keys and values side by side). 16-byte aligned,
+ *                page_stride a multiple of 8. hd 32, 64 or 128; page_size a power of two, 16 to 32768.
+ *  table       : [B][table_stride] int32, of which table_cols entries of a sequence are read: entry
+ *                i is the page of its keys [i * page_size, (i + 1) * page_size). An entry outside
+ *                [0, n_pages) names no page: nothing is written to or read from it.
+ *  seq_start   : [B + 1] int32 ascending: the new tokens of sequence b are the rows
+ *                [seq_start[b], seq_start[b + 1]) of the token arrays (none is allowed). Rows from
+ *                seq_start[B] on belong to no sequence: nothing is written for them.
+ *  kv_len      : [B] int32: keys of sequence b, its new tokens' among them: row i of its n new
+ *                rows is key kv_len[b] - n + i. Keys past table_cols * page_size do not exist. */
+typedef struct gsvk_paged_kv {
+    void * k;
+    void * v;
+    int type;
+    int n_kv;
+    int hd;
+    int page_size;
+    int64_t n_pages;
+    int64_t page_stride;
+    const int32_t * table;
+    int64_t table_stride;
+    int table_cols;
+    int B;
+    const int32_t * seq_start;
+    const int32_t * kv_len;
+} gsvk_paged_kv;
+
+/* The rotation of queries and keys to their positions, as tables of fp32 angles' cosines and sines
+ * ([rows][rot / 2] each, row = position): of the first `rot` elements of each head (a multiple of
+ * 16, at most hd) the pair (i, j) becomes (x_i cos - x_j sin, x_j cos + x_i sin). pairs = 0: i and
+ * j = i + rot / 2, angle i; pairs = 1: 2 i and 2 i + 1, angle i. pos: [tokens] int32 positions, or
+ * NULL: the position of a row is its key index. */
+typedef struct gsvk_rope {
+    const float * cos;
+    const float * sin;
+    int64_t rows;
+    int rot;
+    int pairs;
+    const int32_t * pos;
+} gsvk_rope;
+
+/* Append the keys and values of `tokens` new rows to the cache, keys and queries rotated on the
+ * way (rope NULL: not rotated). q [tokens][nh][hd], k, v [tokens][n_kv][hd] of x_type (GSVK_TYPE_F32
+ * or the cache's type), q_stride / k_stride / v_stride elements from one row to the next (views
+ * into the rows of a fused projection; rows 16-byte aligned). Computed in fp32, rounded once to the
+ * cache's type. The rotated queries go to q_out [tokens][nh][hd] of the cache's type, which may be q
+ * itself where both are dense and of one type; q and q_out NULL (nh 0): keys and values only.
+ * A row whose key has no page, a negative index or a position outside [0, rope->rows) is not
+ * written (q_out neither) and counted in *n_bad (device int32, added to; may be NULL). Two rows of
+ * one call must not name the same slot. k_out, v_out of other slots keep what they held.
+ * Stands for the append of src/gsv_ar.cpp:398-399, there into a dense cache without rotation. */
+int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, const void * k, const void * v, int x_type,
+                         int64_t tokens, int nh, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                         const gsvk_rope * rope, void * q_out, int32_t * n_bad, void * stream);
+
+/* Attention of the new tokens over the pages of their sequences, their own keys (appended before)
+ * among them. q [tokens][nh][hd] of the cache's type, q_stride elements from row to row; query head
+ * h reads key/value head h / (nh / n_kv). A row at key index p sees the keys j of its sequence with
+ *   j < max(p + 1, prefix[b])   (prefix [B] int32: this many first keys are seen by every row, the
+ *                                text part of src/gsv_ar.cpp:215-223; NULL = 0, causal), and
+ *   j > p - window              (window 0: no lower bound),
+ * that exist and lie on a page. out = softmax(scale * q . k) . v in fp32 accumulation, the
+ * probabilities rounded to the cache's type for the matrix cores; written to out [tokens][nh][hd] of
+ * out_type (GSVK_TYPE_F32 or the cache's type), out_stride elements from row to row. lse (may be
+ * NULL) [tokens][nh] fp32: the natural logarithm of the sum of the exponentials. A row that sees no
+ * key gives zeros and -inf. What a row does not see has no effect on it, whatever it holds
+ * (infinities and NaN too).
+ * max_new: the most new tokens of any sequence (rows past it are not computed); max_keys: the most
+ * keys of any sequence, which only decides how the work is split. scale > 0.
+ * ws: gsvk_attn_paged_workspace_bytes() bytes of device memory of the same arguments (NULL if 0);
+ * nothing in it outlives the call. Results do not depend on what else runs, and are the same bits
+ * for the same arguments. */
+size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new,
+                                       int64_t max_keys);
+int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
+                       int max_new, int64_t max_keys, float scale, int window, const int32_t * prefix,
+                       void * out, int out_type, int64_t out_stride, float * lse, void * ws, size_t ws_bytes,
+                       void * stream);
+
 /* ======================================================================================
  * 3. BERT text encoder (src/gsv_bert.{h,cpp}: chinese-roberta-wwm-ext-large, post-LN, the
  *    features the AR prefill takes as a request's `bert` input)
