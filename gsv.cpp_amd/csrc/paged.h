@@ -36,6 +36,8 @@ __device__ __forceinline__ void pg_unpack8(const uint4 & u, float (&x)[8]) {
     }
 }
 
+constexpr int PG_MAX_KEYS = INT32_MAX - 255;
+
 // gsvk_paged_kv as the kernels take it. Everything that comes from device memory is checked where
 // it is read: row ranges are cut to [0, tokens), page numbers to the cache.
 struct PagedView {
@@ -58,10 +60,12 @@ struct PagedView {
         const int64_t s = seq_start[b];
         return s < 0 ? 0 : s > tokens ? tokens : s;
     }
-    // keys of sequence b that the table has room for
-    __device__ __forceinline__ int64_t keys(int b) const {
-        const int64_t n = kv_len[b], cap = (int64_t) table_cols << page_shift;
-        return n < 0 ? 0 : n > cap ? cap : n;
+    // keys of sequence b that the table has room for (sums of a key and a tile stay in 31 bits)
+    __device__ __forceinline__ int keys(int b) const {
+        int64_t n = kv_len[b];
+        const int64_t cap = (int64_t) table_cols << page_shift;
+        n = n < 0 ? 0 : n > cap ? cap : n;
+        return n > PG_MAX_KEYS ? PG_MAX_KEYS : (int) n;
     }
 };
 

@@ -1,11 +1,55 @@
-// Attention of new tokens over a cache in pages (gsvk_op_attn_paged), for gfx950: one wave per
-// (row, query head), the keys in turn, an online softmax per group of lanes.
+// Attention of new tokens over a cache in pages (gsvk_op_attn_paged), for gfx950.
+//
+// Rows. The query heads that share a key/value head are rows of one product: of the n new tokens
+// of a sequence, row r = token r / G, head r % G of the group of G. A row at key index p sees
+// [max(0, p - window + 1), min(keys, max(p + 1, prefix))); both ends grow with the token, so a
+// tile's first and last row give its ranges.
+//
+// Both kernels form the scores transposed, S^T[key][row] = K . Q^T, so that a lane holds one row
+// and several keys: the softmax of a row is in-lane work plus an exchange with the lanes that hold
+// its other keys, and the registers of P^T are the operand of O^T[dim][row] += V^T . P^T as they
+// are (the keys of a step in the order of the score registers; V^T is read from LDS in that order
+// by the transposing 16-bit read, four keys of one dim per lane).
+//
+//   k_attn_paged_few    sequences of at most 32 rows (single tokens, drafts): the keys are dealt to
+//                       the 4 waves of a workgroup in blocks of 32, each wave with its own running
+//                       maximum and sum; K goes straight into the operand registers
+//                       (v_mfma_f32_16x16x32: 16 keys x 32 dims), V through a tile of LDS that
+//                       belongs to the wave, so the loop has no barrier. Bound by HBM.
+//   k_attn_paged_chunk  longer chunks: 8 waves of 32 rows share key tiles of 64 in LDS (double
+//                       buffered), v_mfma_f32_32x32x16.
+// Where a launch would hold too few workgroups, each (sequence, head, row tile) is cut into nsplit
+// runs of keys, whose (maximum, sum, unnormalised output) k_attn_paged_merge joins.
+//
+// Softmax. Exponents are base 2. The reference exponent m of a row is not its running maximum but
+// follows it: it is moved (and O, l rescaled) only when a score exceeds it by more than 2^12, to
+// 2^4 above. Sums and outputs are relative to m throughout, so the result is that of any m;
+// probabilities stay below 2^12, in range of fp16, and those far below the maximum are kept from
+// its subnormals. They are rounded to the cache's type for the product (half a step each, random
+// in sign: on the output about as much again as its own rounding); l sums them unrounded.
+//
+// What a row does not see must not reach it. Scores of unseen keys are replaced by -inf. Values
+// of keys that no row of the tile sees are replaced by zeros on their way to LDS. Where some rows
+// of a tile see a key and others do not, 0 * inf would still give NaN: such blocks are searched
+// for infinities and NaNs, which are taken out of the product and added one by one (rare).
+#include <cfloat>
 #include <cmath>
 
 #include "paged.h"
 
 namespace gsvk {
 namespace {
+
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16 __attribute__((ext_vector_type(16)));
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) pg_s4 pg_lds4;
+
+constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
+constexpr int FEW_WAVES = 4, FEW_KEYS = 32;
+constexpr int CH_WAVES = 8, CH_KEYS = 64;
+constexpr float M_NONE = -FLT_MAX;    // m of a row that has seen nothing: exp2(score - m) of -inf is 0
+constexpr float M_ROOM = 12.0f, M_SET = 4.0f;
 
 struct PagedAttn {
     PagedView kv;
@@ -15,97 +59,725 @@ struct PagedAttn {
     int64_t out_stride;   // elements
     float * lse;
     const int32_t * prefix;
+    float * part_o;     // [nsplit][tokens * nh][HD]
+    float * part_ml;    // [nsplit][tokens * nh][2]
     float scale_log2;
     int group;   // query heads per key/value head
     int window;
     int max_new;
+    int out_f32;
+    int nsplit;       // of this launch
+    int min_rows;     // sequences of fewer rows are another launch's
+    int max_rows;     // and of more
 };
 
-// Wave of (row, head): HD / 8 lanes share a key, each holding 8 dims; the groups of lanes keep
-// their own running maximum and sum and are joined at the end.
-template <class T, int HD, bool F32OUT>
-__global__ void __launch_bounds__(64) k_attn_paged_rows(PagedAttn a) {
-    constexpr int LK = HD / 8, KI = 64 / LK;
-    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63;
-    const int64_t r0 = a.kv.row0(b), r1 = a.kv.row0(b + 1);
-    const int64_t row = r0 + blockIdx.x;
-    if (row >= r1) return;
-    const int64_t len = a.kv.keys(b);
-    const int64_t p = (int64_t) a.kv.kv_len[b] - (r1 - row);
-    int64_t hi = p + 1, lo = 0;
-    if (a.prefix && a.prefix[b] > hi) hi = a.prefix[b];
-    if (hi > len) hi = len;
-    if (a.window && p - a.window + 1 > 0) lo = p - a.window + 1;
+template <class T>
+__device__ __forceinline__ pg_f4 mfma16(typename T::v8 a, typename T::v8 b, pg_f4 c) {
+    if constexpr (__is_same(T, PgF16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <class T>
+__device__ __forceinline__ pg_f16 mfma32(typename T::v8 a, typename T::v8 b, pg_f16 c) {
+    if constexpr (__is_same(T, PgF16)) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
 
-    const int sub = lane % LK, kg = lane / LK;
-    float q[8];
-    pg_unpack8<T>(*reinterpret_cast<const uint4 *>(a.q + row * a.q_stride + h * HD + sub * 8), q);
-    float m = -INFINITY, l = 0.0f, o[8] = {};
-    for (int64_t j0 = lo; j0 < hi; j0 += KI) {
-        const int64_t j = j0 + kg;
-        int64_t page = -1;
-        if (j < hi) page = a.kv.table[b * a.kv.table_stride + (j >> a.kv.page_shift)];
-        const bool see = page >= 0 && page < a.kv.n_pages;
-        const int64_t at = (see ? page : 0) * a.kv.page_stride
-                           + (((int64_t) (h / a.group) << a.kv.page_shift) + (j & ((1 << a.kv.page_shift) - 1))) * HD + sub * 8;
-        float x[8], s = 0.0f;
-        pg_unpack8<T>(*reinterpret_cast<const uint4 *>(a.kv.k + at), x);
+// Transposing LDS read: the 16 lanes of a group give the addresses of 4 rows x 16 columns of
+// 16-bit values (lane i: row i / 4, columns 4 (i % 4) .. + 3), lane i receives column i of the 4 rows.
+__device__ __forceinline__ uint2 lds_tr4(const uint16_t * p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((pg_lds4 *) p));
+}
+template <class T>
+__device__ __forceinline__ typename T::v8 v8_of(uint2 a, uint2 b) {
+    return __builtin_bit_cast(typename T::v8, make_uint4(a.x, a.y, b.x, b.y));
+}
+template <class T>
+__device__ __forceinline__ typename T::v8 v8_of(const uint4 & a) { return __builtin_bit_cast(typename T::v8, a); }
+
+// max / sum with the lane 32 away
+__device__ __forceinline__ float max_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Swizzles of 16-byte pieces inside a key's LDS row of HD values, so that the rows that one read
+// touches fall in different banks (256 bytes): for V pairs of pieces (the transposing read takes 32
+// bytes of 4 keys), for K single ones (16 bytes of 16 keys).
+template <int HD>
+__device__ __forceinline__ int swz_v(int key) { return 2 * ((key / (128 / HD)) & (HD / 16 - 1)); }
+template <int HD>
+__device__ __forceinline__ int swz_k(int key) { return (key / (128 / HD)) & (HD / 8 - 1); }
+
+// infinities and NaNs of a pair of 16-bit values: all exponent bits set
+template <class T>
+__device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
+    constexpr uint32_t E = __is_same(T, PgF16) ? 0x7C007C00u : 0x7F807F80u, ONE = E & ~(E << 1);
+    return ((w & E) + ONE) & 0x80008000u;   // (no carry leaves a half: its sign bit was cleared)
+}
+template <class T>
+__device__ __forceinline__ bool any_odd(const uint4 & u) {
+    return (odd_mask<T>(u.x) | odd_mask<T>(u.y) | odd_mask<T>(u.z) | odd_mask<T>(u.w)) != 0;
+}
+template <class T>
+__device__ __forceinline__ void clear_odd(uint4 & u) {
+    uint32_t * w = &u.x;
 #pragma unroll
-        for (int i = 0; i < 8; i++) s = __builtin_fmaf(q[i], x[i], s);
-#pragma unroll
-        for (int d = 1; d < LK; d <<= 1) s += __shfl_xor(s, d, 64);
-        if (!see) continue;
-        s *= a.scale_log2;
-        const float mn = fmaxf(m, s);
-        if (mn == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(m - mn), e = __builtin_amdgcn_exp2f(s - mn);
-        pg_unpack8<T>(*reinterpret_cast<const uint4 *>(a.kv.v + at), x);
-        l = l * f + e;
-#pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = __builtin_fmaf(e, x[i], o[i] * f);
-        m = mn;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t o = odd_mask<T>(w[i]);
+        w[i] &= ~((o >> 15) * 0xffffu);
     }
-    float M = m;
-#pragma unroll
-    for (int d = LK; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-    l *= f;
-#pragma unroll
-    for (int d = LK; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        o[i] *= f;
-#pragma unroll
-        for (int d = LK; d < 64; d <<= 1) o[i] += __shfl_xor(o[i], d, 64);
-        o[i] *= inv;
-    }
-    if (lane >= LK) return;
-    const int64_t at = row * a.out_stride + h * HD + sub * 8;
-    if constexpr (F32OUT) {
-        float * out = (float *) a.out + at;
-        *reinterpret_cast<float4 *>(out) = make_float4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<float4 *>(out + 4) = make_float4(o[4], o[5], o[6], o[7]);
+}
+template <class T>
+__device__ __forceinline__ bool is_odd(uint16_t u) { return odd_mask<T>(u) != 0; }
+
+// What a workgroup works on: its sequence's rows and the key ranges of rows
+struct Seq {
+    int64_t row0;   // first row of the token arrays
+    int n;          // new tokens that are computed
+    int rows;       // n * G
+    int keys;
+    int64_t p0;     // key index of token 0 (may be negative)
+    int prefix;
+};
+
+__device__ __forceinline__ Seq seq_of(const PagedAttn & a, int b) {
+    Seq s;
+    s.row0 = a.kv.row0(b);
+    const int64_t n = a.kv.row0(b + 1) - s.row0;
+    s.keys = a.kv.keys(b);
+    s.p0 = (int64_t) a.kv.kv_len[b] - n;
+    s.n = n < 0 ? 0 : n > a.max_new ? a.max_new : (int) n;
+    s.rows = s.n * a.group;
+    s.prefix = a.prefix ? a.prefix[b] : 0;
+    return s;
+}
+__device__ __forceinline__ int key_lo(const PagedAttn & a, const Seq & s, int tok) {
+    const int64_t lo = s.p0 + tok - a.window + 1;
+    return a.window && lo > 0 ? (int) lo : 0;
+}
+__device__ __forceinline__ int key_hi(const Seq & s, int tok) {
+    int64_t hi = s.p0 + tok + 1;
+    hi = hi > s.prefix ? hi : s.prefix;
+    return hi < 0 ? 0 : hi > s.keys ? s.keys : (int) hi;
+}
+
+// Page of a key (uniform over the wave), -1 if it has none
+__device__ __forceinline__ int page_of(const PagedAttn & a, const int32_t * tb, int key) {
+    const int col = key >> a.kv.page_shift;
+    const int pg = col < a.kv.table_cols ? tb[col] : -1;
+    return pg >= 0 && pg < a.kv.n_pages ? pg : -1;
+}
+// Element offset of key `key` (on page pg; any page if it has none) of head kvh
+template <int HD>
+__device__ __forceinline__ int64_t key_at(const PagedAttn & a, int pg, int kvh, int key) {
+    return (int64_t) max(pg, 0) * a.kv.page_stride
+           + (((int64_t) kvh << a.kv.page_shift) + (key & ((1 << a.kv.page_shift) - 1))) * HD;
+}
+
+// Store 8 output values of a row: final, or a split's unnormalised ones
+template <class T>
+__device__ __forceinline__ void store8(const PagedAttn & a, int64_t row, int col, const float (&x)[8]) {
+    const int64_t at = row * a.out_stride + col;
+    if (a.out_f32) {
+        float4 * o = reinterpret_cast<float4 *>((float *) a.out + at);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]);
+        o[1] = make_float4(x[4], x[5], x[6], x[7]);
     } else {
-        *reinterpret_cast<uint4 *>((uint16_t *) a.out + at) = make_uint4(pg_pack<T>(o[0], o[1]), pg_pack<T>(o[2], o[3]),
-                                                                        pg_pack<T>(o[4], o[5]), pg_pack<T>(o[6], o[7]));
+        *reinterpret_cast<uint4 *>((uint16_t *) a.out + at) = make_uint4(pg_pack<T>(x[0], x[1]), pg_pack<T>(x[2], x[3]),
+                                                                        pg_pack<T>(x[4], x[5]), pg_pack<T>(x[6], x[7]));
     }
-    if (a.lse && lane == 0)
-        a.lse[row * gridDim.y + h] = l != 0.0f ? 0.69314718055994531f * (M + __builtin_log2f(l)) : -INFINITY;
+}
+template <class T>
+__device__ __forceinline__ void store4(const PagedAttn & a, int64_t row, int col, float x, float y, float z, float w) {
+    const int64_t at = row * a.out_stride + col;
+    if (a.out_f32) *reinterpret_cast<float4 *>((float *) a.out + at) = make_float4(x, y, z, w);
+    else *reinterpret_cast<uint2 *>((uint16_t *) a.out + at) = make_uint2(pg_pack<T>(x, y), pg_pack<T>(z, w));
+}
+// natural logarithm of a row's sum (l relative to 2^m)
+__device__ __forceinline__ float lse_of(float m, float l) {
+    return l != 0.0f ? 0.69314718055994531f * (m + __builtin_log2f(l)) : -INFINITY;
+}
+
+// ---- few rows ------------------------------------------------------------------------------------
+
+// QT tiles of 16 rows per workgroup
+template <class T, int HD, int QT>
+__global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) {
+    constexpr int C = HD / 8, NV = FEW_KEYS * C / 64, NK = HD / 32, DT = HD / 16, OS = HD + 4;
+    constexpr int VB = FEW_KEYS * HD * 2, OB = 16 * OS * 4;   // LDS bytes of a wave: V tile, outputs
+    __shared__ __align__(16) char s_mem[FEW_WAVES * (VB > OB ? VB : OB)];
+    __shared__ float s_ml[FEW_WAVES][QT * 16][2];
+
+    const int b = blockIdx.z, kvh = blockIdx.y;
+    const int split = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Seq s = seq_of(a, b);
+    const int r0 = rt * QT * 16;
+    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    const int nh = a.group * a.kv.n_kv;
+    const int tok0 = r0 / a.group, tok1 = min(r0 + QT * 16, s.rows) - 1, tokl = tok1 / a.group;
+    const int klo = key_lo(a, s, tok0), khi = key_hi(s, tokl);
+    const int lo_max = key_lo(a, s, tokl), hi_min = key_hi(s, tok0);
+
+    int lo[QT], hi[QT];
+    typename T::v8 qf[QT][NK];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const int r = min(r0 + t * 16 + li, s.rows - 1), tok = r / a.group, h = kvh * a.group + r % a.group;
+        lo[t] = key_lo(a, s, tok);
+        hi[t] = key_hi(s, tok);
+        const uint16_t * qp = a.q + (s.row0 + tok) * a.q_stride + h * HD + 8 * lg;
+#pragma unroll
+        for (int c = 0; c < NK; c++) qf[t][c] = v8_of<T>(*reinterpret_cast<const uint4 *>(qp + 32 * c));
+    }
+
+    // the run of key blocks of this split, dealt to the waves in turn
+    const int blk_a = klo / FEW_KEYS, nblk = khi > klo ? (khi + FEW_KEYS - 1) / FEW_KEYS - blk_a : 0;
+    const int per = (nblk + a.nsplit - 1) / a.nsplit;
+    const int blk0 = blk_a + min(nblk, split * per), blk1 = blk_a + min(nblk, (split + 1) * per);
+
+    const int32_t * tb = a.kv.table + b * a.kv.table_stride;
+    uint16_t * sv = reinterpret_cast<uint16_t *>(s_mem + wave * VB);
+    uint4 kr[2][NK], vr[NV];
+    int pg[2];
+    const auto fetch = [&](int blk, const int (&p)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int64_t at = key_at<HD>(a, p[t], kvh, blk * FEW_KEYS + 16 * t);
+            const uint16_t * kp = a.kv.k + at + li * HD + 8 * lg;
+            const uint16_t * vp = a.kv.v + at + lane * 8;
+#pragma unroll
+            for (int c = 0; c < NK; c++) kr[t][c] = *reinterpret_cast<const uint4 *>(kp + 32 * c);
+#pragma unroll
+            for (int i = 0; i < NV / 2; i++) vr[t * (NV / 2) + i] = *reinterpret_cast<const uint4 *>(vp + i * 512);
+        }
+    };
+
+    float m[QT], l[QT];
+    pg_f4 o[QT][DT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        m[t] = M_NONE;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[t][d] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int blk = blk0 + wave;
+    if (blk < blk1) {
+        pg[0] = page_of(a, tb, blk * FEW_KEYS);
+        pg[1] = page_of(a, tb, blk * FEW_KEYS + 16);
+        fetch(blk, pg);
+    }
+    for (; blk < blk1; blk += FEW_WAVES) {
+        const int kb = blk * FEW_KEYS;
+        const bool ok0 = pg[0] >= 0, ok1 = pg[1] >= 0;
+        const bool full = kb >= lo_max && kb + FEW_KEYS <= hi_min && ok0 && ok1;
+        // the next block's pages
+        const int nb = blk + FEW_WAVES < blk1 ? blk + FEW_WAVES : blk;
+        const int np[2] = {page_of(a, tb, nb * FEW_KEYS), page_of(a, tb, nb * FEW_KEYS + 16)};
+        bool odd = false;
+        if (!full) {
+            const bool ragged = lo_max > klo || hi_min < khi;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int key = kb + (i * 64 + lane) / C;
+                const bool see = key >= klo && key < khi && (i < NV / 2 ? ok0 : ok1);
+                if (!see) vr[i] = make_uint4(0, 0, 0, 0);
+                if (ragged) odd |= any_odd<T>(vr[i]);
+            }
+            odd = __any(odd);
+            if (odd)
+#pragma unroll
+                for (int i = 0; i < NV; i++) clear_odd<T>(vr[i]);
+        }
+        // scores
+        pg_f4 sc[QT][2];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                sc[t][k] = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < NK; c++) sc[t][k] = mfma16<T>(v8_of<T>(kr[k][c]), qf[t][c], sc[t][k]);
+            }
+        // V into the wave's LDS tile, the next block on its way
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int u = i * 64 + lane, key = u / C;
+            *reinterpret_cast<uint4 *>(sv + key * HD + (((u % C) ^ swz_v<HD>(key)) << 3)) = vr[i];
+        }
+        pg[0] = np[0];
+        pg[1] = np[1];
+        fetch(nb, pg);
+        typename T::v8 pf[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const int key = kb + 16 * k + 4 * lg + v;
+                        if (!(key >= lo[t] && key < hi[t] && (k ? ok1 : ok0))) sc[t][k][v] = -INFINITY;
+                    }
+            }
+            float top = fmaxf(fmaxf(fmaxf(sc[t][0][0], sc[t][0][1]), fmaxf(sc[t][0][2], sc[t][0][3])),
+                              fmaxf(fmaxf(sc[t][1][0], sc[t][1][1]), fmaxf(sc[t][1][2], sc[t][1][3])));
+            top *= a.scale_log2;
+            if (__any(top > m[t] + M_ROOM)) {
+                top = max_x32(fmaxf(top, __shfl_xor(top, 16, 64)));
+                const float mn = fmaxf(m[t], top - M_SET);
+                const float f = __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[t][d] *= f;
+            }
+            float p[8], sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v >> 2][v & 3], a.scale_log2, -m[t]));
+                sum += p[v];
+                sc[t][v >> 2][v & 3] = p[v];
+            }
+            l[t] += sum;
+            pf[t] = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
+                                        pg_pack<T>(p[6], p[7])));
+        }
+        // O^T += V^T . P^T, keys 4 g + .. of both halves
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int key = 4 * lg + (li >> 2), ch = 2 * d + ((li & 3) >> 1);
+            const uint16_t * p = sv + key * HD + ((ch ^ swz_v<HD>(key)) << 3) + 4 * (li & 1);
+            const uint16_t * p2 = sv + (key + 16) * HD + ((ch ^ swz_v<HD>(key + 16)) << 3) + 4 * (li & 1);
+            const typename T::v8 vf = v8_of<T>(lds_tr4(p), lds_tr4(p2));
+#pragma unroll
+            for (int t = 0; t < QT; t++) o[t][d] = mfma16<T>(vf, pf[t], o[t][d]);
+        }
+        if (odd) {   // the infinities and NaNs that some of the rows see
+            for (int j = 0; j < FEW_KEYS; j++) {
+                const int key = kb + j, page = page_of(a, tb, key);
+                if (page < 0 || key < klo || key >= khi) continue;
+                const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lg;
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < 8; v++) mine = (j >> 4) * 4 + (j & 3) == v ? sc[t][v >> 2][v & 3] : mine;
+                    const float p = __shfl(mine, li + 16 * ((j & 15) >> 2), 64);
+                    const bool see = key >= lo[t] && key < hi[t];
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint16_t u = vp[16 * d + e];
+                            if (see && is_odd<T>(u)) o[t][d][e] += p * T::up(u);
+                        }
+                }
+            }
+        }
+    }
+
+    // join the waves
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        l[t] = sum_x32(l[t] + __shfl_xor(l[t], 16, 64));
+        if (lg == 0) {
+            s_ml[wave][t * 16 + li][0] = m[t];
+            s_ml[wave][t * 16 + li][1] = l[t];
+        }
+    }
+    __syncthreads();
+    float * so = reinterpret_cast<float *>(s_mem);
+    for (int t = 0; t < QT; t++) {
+        if (t) __syncthreads();
+        float M = s_ml[0][t * 16 + li][0];
+#pragma unroll
+        for (int w = 1; w < FEW_WAVES; w++) M = fmaxf(M, s_ml[w][t * 16 + li][0]);
+        const float f = __builtin_amdgcn_exp2f(s_ml[wave][t * 16 + li][0] - M);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            pg_f4 x = QT == 1 || t == 0 ? o[0][d] : o[QT - 1][d];
+            x *= f;
+            *reinterpret_cast<pg_f4 *>(so + (wave * 16 + li) * OS + 16 * d + 4 * lg) = x;
+        }
+        __syncthreads();
+        // a thread: 8 dims of a row
+        const int rr = tid / C, col = (tid % C) * 8, r = r0 + t * 16 + rr;
+        if (rr < 16 && r < s.rows) {
+            const int tok = r / a.group, h = kvh * a.group + r % a.group;
+            float Mr = M_NONE, L = 0.0f, x[8] = {};
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; w++) Mr = fmaxf(Mr, s_ml[w][t * 16 + rr][0]);
+#pragma unroll
+            for (int w = 0; w < FEW_WAVES; w++) {
+                L += s_ml[w][t * 16 + rr][1] * __builtin_amdgcn_exp2f(s_ml[w][t * 16 + rr][0] - Mr);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] += so[(w * 16 + rr) * OS + col + i];
+            }
+            const int64_t row = s.row0 + tok, id = row * nh + h;
+            if (a.nsplit == 1) {
+                const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
+                store8<T>(a, row, h * HD + col, x);
+                if (a.lse && col == 0) a.lse[id] = lse_of(Mr, L);
+            } else {
+                const int64_t at = (int64_t) split * a.kv.tokens * nh + id;
+                float4 * po = reinterpret_cast<float4 *>(a.part_o + at * HD + col);
+                po[0] = make_float4(x[0], x[1], x[2], x[3]);
+                po[1] = make_float4(x[4], x[5], x[6], x[7]);
+                if (col == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(Mr, L);
+            }
+        }
+    }
+}
+
+// ---- chunks ----------------------------------------------------------------------------------------
+
+template <class T, int HD>
+__global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn a) {
+    constexpr int C = HD / 8, NT = CH_WAVES * 64, UNITS = CH_KEYS * C, NU = 2 * UNITS / NT;
+    constexpr int NK = HD / 16, DT = HD / 32;
+    __shared__ __align__(16) uint16_t s_k[2][CH_KEYS * HD];
+    __shared__ __align__(16) uint16_t s_v[2][CH_KEYS * HD];
+    __shared__ int s_odd[2];
+
+    const int b = blockIdx.z, kvh = blockIdx.y;
+    const int split = blockIdx.x % a.nsplit;
+    const int rt = gridDim.x / a.nsplit - 1 - blockIdx.x / a.nsplit;   // the last rows see the most keys: first
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, lh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Seq s = seq_of(a, b);
+    const int r0 = rt * CH_WAVES * 32;
+    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    const int nh = a.group * a.kv.n_kv;
+    // the key range of the workgroup and of this wave
+    const int tokf = r0 / a.group, tokl = (min(r0 + CH_WAVES * 32, s.rows) - 1) / a.group;
+    const int klo = key_lo(a, s, tokf), khi = key_hi(s, tokl);
+    const bool ragged = key_lo(a, s, tokl) > klo || key_hi(s, tokf) < khi;
+    const int rw = r0 + wave * 32;
+    const bool idle = rw >= s.rows;
+    const int tw0 = min(rw, s.rows - 1) / a.group, tw1 = min(rw + 31, s.rows - 1) / a.group;
+    const int wlo = key_lo(a, s, tw0), wlo_max = key_lo(a, s, tw1), whi_min = key_hi(s, tw0), whi = key_hi(s, tw1);
+    const int r = min(rw + li, s.rows - 1), tok = r / a.group, h = kvh * a.group + r % a.group;
+    const int lo = key_lo(a, s, tok), hi = key_hi(s, tok);
+
+    typename T::v8 qf[NK];
+    {
+        const uint16_t * qp = a.q + (s.row0 + tok) * a.q_stride + h * HD + 8 * lh;
+#pragma unroll
+        for (int c = 0; c < NK; c++) qf[c] = v8_of<T>(*reinterpret_cast<const uint4 *>(qp + 16 * c));
+    }
+    const int kt_a = klo / CH_KEYS, nkt = khi > klo ? (khi + CH_KEYS - 1) / CH_KEYS - kt_a : 0;
+    const int per = (nkt + a.nsplit - 1) / a.nsplit;
+    const int kt0 = kt_a + min(nkt, split * per), kt1 = kt_a + min(nkt, (split + 1) * per);
+
+    const int32_t * tb = a.kv.table + b * a.kv.table_stride;
+    // pages of a tile's four groups of 16 keys
+    struct Pages { int p[CH_KEYS / 16]; };
+    const auto pages = [&](int kt) {
+        Pages g;
+#pragma unroll
+        for (int i = 0; i < CH_KEYS / 16; i++) g.p[i] = page_of(a, tb, kt * CH_KEYS + 16 * i);
+        return g;
+    };
+    // A thread's 16-byte units of a tile: K first, then V, in the order of the keys; the 64 units of a
+    // wave lie in one group of 16 keys.
+    uint4 st[NU];
+    const auto fetch = [&](int kt, const Pages & g) {
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int w0 = i * NT + wave * 64, uu = w0 % UNITS, kg = uu / C / 16;
+            const int pg = kg == 0 ? g.p[0] : kg == 1 ? g.p[1] : kg == 2 ? g.p[2] : g.p[3];
+            const int64_t at = key_at<HD>(a, pg, kvh, kt * CH_KEYS + 16 * kg) + (uu - kg * 16 * C) * 8;
+            st[i] = *reinterpret_cast<const uint4 *>((w0 < UNITS ? a.kv.k : a.kv.v) + at + lane * 8);
+        }
+    };
+    const auto stage = [&](int kt, const Pages & g, int buf) {
+#pragma unroll
+        for (int i = 0; i < NU; i++) {
+            const int w0 = i * NT + wave * 64, uu = w0 % UNITS, kg = uu / C / 16;
+            const int u = uu + lane, key = u / C;
+            if (w0 < UNITS) {
+                *reinterpret_cast<uint4 *>(&s_k[buf][key * HD + (((u % C) ^ swz_k<HD>(key)) << 3)]) = st[i];
+            } else {
+                const int pg = kg == 0 ? g.p[0] : kg == 1 ? g.p[1] : kg == 2 ? g.p[2] : g.p[3];
+                const int at = kt * CH_KEYS + key;
+                if (!(pg >= 0 && at >= klo && at < khi)) st[i] = make_uint4(0, 0, 0, 0);
+                if (ragged && any_odd<T>(st[i])) {
+                    clear_odd<T>(st[i]);
+                    s_odd[buf] = kt + 1;
+                }
+                *reinterpret_cast<uint4 *>(&s_v[buf][key * HD + (((u % C) ^ swz_v<HD>(key)) << 3)]) = st[i];
+            }
+        }
+    };
+
+    float m = M_NONE, l = 0.0f;
+    pg_f16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+
+    if (tid < 2) s_odd[tid] = 0;
+    __syncthreads();
+    Pages cur{}, nxt{};
+    if (kt0 < kt1) {
+        cur = pages(kt0);
+        fetch(kt0, cur);
+        stage(kt0, cur, 0);
+        nxt = pages(min(kt0 + 1, kt1 - 1));
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int kt = kt0; kt < kt1; kt++, buf ^= 1) {
+        const bool more = kt + 1 < kt1;
+        if (more) fetch(kt + 1, nxt);
+        const Pages nn = pages(min(kt + 2, kt1 - 1));
+        const int kb = kt * CH_KEYS;
+        const bool okp = cur.p[0] >= 0 && cur.p[1] >= 0 && cur.p[2] >= 0 && cur.p[3] >= 0;
+        if (!idle && kb < whi && kb + CH_KEYS > wlo) {
+            const bool full = kb >= wlo_max && kb + CH_KEYS <= whi_min && okp;
+            pg_f16 sc[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) sc[k][v] = 0.0f;
+                const int key = 32 * k + li;
+#pragma unroll
+                for (int c = 0; c < NK; c++) {
+                    const uint4 kf = *reinterpret_cast<const uint4 *>(&s_k[buf][key * HD + (((2 * c + lh) ^ swz_k<HD>(key)) << 3)]);
+                    sc[k] = mfma32<T>(v8_of<T>(kf), qf[c], sc[k]);
+                }
+            }
+            if (!full) {
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) {
+                        const int j = 32 * k + 8 * (v >> 2) + 4 * lh + (v & 3);
+                        if (!(kb + j >= lo && kb + j < hi && cur.p[2 * k + (v >> 3)] >= 0)) sc[k][v] = -INFINITY;
+                    }
+            }
+            float top = fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+            for (int v = 1; v < 16; v++) top = fmaxf(fmaxf(top, sc[0][v]), sc[1][v]);
+            top *= a.scale_log2;
+            if (__any(top > m + M_ROOM)) {
+                const float mn = fmaxf(m, max_x32(top) - M_SET);
+                const float f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[d][v] *= f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    sc[k][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][v], a.scale_log2, -m));
+                    sum += sc[k][v];
+                }
+            l += sum;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const int v0 = 8 * c;
+                    const typename T::v8 pf = v8_of<T>(make_uint4(
+                        pg_pack<T>(sc[k][v0], sc[k][v0 + 1]), pg_pack<T>(sc[k][v0 + 2], sc[k][v0 + 3]),
+                        pg_pack<T>(sc[k][v0 + 4], sc[k][v0 + 5]), pg_pack<T>(sc[k][v0 + 6], sc[k][v0 + 7])));
+                    const int key = 32 * k + 16 * c + 4 * lh + ((lane & 15) >> 2);
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                        const uint16_t * p = &s_v[buf][key * HD + ((ch ^ swz_v<HD>(key)) << 3) + 4 * (lane & 1)];
+                        const uint16_t * p2 = &s_v[buf][(key + 8) * HD + ((ch ^ swz_v<HD>(key + 8)) << 3) + 4 * (lane & 1)];
+                        o[d] = mfma32<T>(v8_of<T>(lds_tr4(p), lds_tr4(p2)), pf, o[d]);
+                    }
+                }
+            if (s_odd[buf] == kt + 1) {   // the infinities and NaNs that some of the rows see
+                for (int j = 0; j < CH_KEYS; j++) {
+                    const int key = kb + j, page = page_of(a, tb, key);
+                    if (page < 0 || key < klo || key >= khi) continue;
+                    const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lh;
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int v = 0; v < 32; v++)
+                        mine = (j >> 5) * 16 + ((j >> 3) & 3) * 4 + (j & 3) == v ? sc[v >> 4][v & 15] : mine;
+                    const float p = __shfl(mine, li + 32 * ((j >> 2) & 1), 64);
+                    const bool see = key >= lo && key < hi;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int v = 0; v < 16; v++) {
+                            const uint16_t u = vp[32 * d + 8 * (v >> 2) + (v & 3)];
+                            if (see && is_odd<T>(u)) o[d][v] += p * T::up(u);
+                        }
+                }
+            }
+        }
+        if (more) stage(kt + 1, nxt, buf ^ 1);
+        cur = nxt;
+        nxt = nn;
+        __syncthreads();
+    }
+
+    if (idle) return;
+    l = sum_x32(l);
+    if (rw + li >= s.rows) return;
+    const int64_t row = s.row0 + tok, id = row * nh + h;
+    if (a.nsplit == 1) {
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                pg_f4 x = {o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
+                x *= inv;
+                if (l == 0.0f) x = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
+                store4<T>(a, row, h * HD + 32 * d + 2 * v + 4 * lh, x[0], x[1], x[2], x[3]);
+            }
+        if (a.lse && lh == 0) a.lse[id] = lse_of(m, l);
+    } else {
+        const int64_t at = (int64_t) split * a.kv.tokens * nh + id;
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4)
+                *reinterpret_cast<float4 *>(a.part_o + at * HD + 32 * d + 2 * v + 4 * lh) =
+                    make_float4(o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]);
+        if (lh == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(m, l);
+    }
+}
+
+// ---- joining the splits ------------------------------------------------------------------------------
+
+// A workgroup: 16 rows of one (sequence, head); a thread 8 dims of a row at a time
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
+    constexpr int C = HD / 8;
+    const int b = blockIdx.z, kvh = blockIdx.y;
+    const Seq s = seq_of(a, b);
+    const int r0 = blockIdx.x * 16;
+    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    const int rr = threadIdx.x / C, col = (threadIdx.x % C) * 8, r = r0 + rr;
+    if (rr >= 16 || r >= s.rows) return;
+    const int nh = a.group * a.kv.n_kv, tok = r / a.group, h = kvh * a.group + r % a.group;
+    const int64_t row = s.row0 + tok, id = row * nh + h, step = a.kv.tokens * nh;
+    float M = M_NONE, L = 0.0f, x[8] = {};
+    for (int i = 0; i < a.nsplit; i++) M = fmaxf(M, a.part_ml[2 * (i * step + id)]);
+    for (int i = 0; i < a.nsplit; i++) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (i * step + id));
+        const float f = __builtin_amdgcn_exp2f(ml.x - M);
+        const float4 * p = reinterpret_cast<const float4 *>(a.part_o + (i * step + id) * HD + col);
+        const float4 u = p[0], w = p[1];
+        L = __builtin_fmaf(ml.y, f, L);
+        x[0] = __builtin_fmaf(u.x, f, x[0]); x[1] = __builtin_fmaf(u.y, f, x[1]);
+        x[2] = __builtin_fmaf(u.z, f, x[2]); x[3] = __builtin_fmaf(u.w, f, x[3]);
+        x[4] = __builtin_fmaf(w.x, f, x[4]); x[5] = __builtin_fmaf(w.y, f, x[5]);
+        x[6] = __builtin_fmaf(w.z, f, x[6]); x[7] = __builtin_fmaf(w.w, f, x[7]);
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
+    store8<T>(a, row, h * HD + col, x);
+    if (a.lse && col == 0) a.lse[id] = lse_of(M, L);
+}
+
+// ---- the host's side -----------------------------------------------------------------------------------
+
+// How a call is cut: a function of its arguments alone (the workspace's size follows from it)
+struct Plan {
+    bool few, chunk;
+    int few_qt, few_tiles, few_split;
+    int chunk_tiles, chunk_split;
+};
+
+int split_for(int64_t workgroups, int64_t want, int64_t max_keys, int64_t least) {
+    int64_t n = (want + workgroups - 1) / workgroups;
+    const int64_t most = max_keys / least;
+    if (n > most) n = most;
+    if (n > 64) n = 64;
+    return n < 1 ? 1 : (int) n;
+}
+
+Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t max_keys) {
+    Plan p{};
+    if (max_new > tokens) max_new = (int) tokens;
+    const int64_t rows = (int64_t) max_new * group;
+    p.chunk = rows > FEW_ROWS;
+    p.few = !p.chunk || (B > 1 && group <= FEW_ROWS);
+    if (p.few) {
+        const int64_t most = rows < FEW_ROWS ? rows : FEW_ROWS;
+        p.few_qt = most <= 16 || (p.chunk && group <= 16) ? 1 : 2;
+        p.few_tiles = (int) ((most + 16 * p.few_qt - 1) / (16 * p.few_qt));
+        p.few_split = split_for((int64_t) B * n_kv, 1024, max_keys, 256);
+    }
+    if (p.chunk) {
+        constexpr int R = CH_WAVES * 32;
+        p.chunk_tiles = (int) ((rows + R - 1) / R);
+        int64_t tiles = tokens * group / R;   // of all sequences, about
+        if (tiles < 1) tiles = 1;
+        p.chunk_split = split_for(tiles * n_kv, 256, max_keys, 512);
+    }
+    return p;
 }
 
 template <class T, int HD>
-void launch_attn(const PagedAttn & a, int nh, bool f32, hipStream_t st) {
-    const dim3 grid((unsigned) a.max_new, (unsigned) nh, (unsigned) a.kv.B);
-    if (f32) hipLaunchKernelGGL((k_attn_paged_rows<T, HD, true>), grid, dim3(64), 0, st, a);
-    else hipLaunchKernelGGL((k_attn_paged_rows<T, HD, false>), grid, dim3(64), 0, st, a);
+void launch_attn(PagedAttn a, const Plan & p, hipStream_t st) {
+    const unsigned nkv = (unsigned) a.kv.n_kv, B = (unsigned) a.kv.B;
+    const auto merge = [&](int rows) {
+        if (a.nsplit > 1)
+            hipLaunchKernelGGL((k_attn_paged_merge<T, HD>), dim3((unsigned) ((rows + 15) / 16), nkv, B), dim3(256), 0, st, a);
+    };
+    if (p.chunk) {
+        a.nsplit = p.chunk_split;
+        a.min_rows = p.few ? FEW_ROWS + 1 : 1;
+        a.max_rows = INT32_MAX;
+        hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) (p.chunk_tiles * p.chunk_split), nkv, B),
+                           dim3(CH_WAVES * 64), 0, st, a);
+        merge(a.max_new * a.group);
+    }
+    if (p.few) {
+        a.nsplit = p.few_split;
+        a.min_rows = 1;
+        a.max_rows = FEW_ROWS;
+        const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
+        if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1>), grid, dim3(FEW_WAVES * 64), 0, st, a);
+        else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2>), grid, dim3(FEW_WAVES * 64), 0, st, a);
+        merge(FEW_ROWS);
+    }
 }
 
 template <class T>
-void launch_attn(const PagedAttn & a, int hd, int nh, bool f32, hipStream_t st) {
-    if (hd == 32) launch_attn<T, 32>(a, nh, f32, st);
-    else if (hd == 64) launch_attn<T, 64>(a, nh, f32, st);
-    else launch_attn<T, 128>(a, nh, f32, st);
+void launch_attn(const PagedAttn & a, int hd, const Plan & p, hipStream_t st) {
+    if (hd == 32) launch_attn<T, 32>(a, p, st);
+    else if (hd == 64) launch_attn<T, 64>(a, p, st);
+    else launch_attn<T, 128>(a, p, st);
+}
+
+// bytes of a split's partial results: rows x (HD outputs, maximum, sum)
+size_t workspace_of(const Plan & p, int64_t rows, int hd) {
+    int n = 1;
+    if (p.few && p.few_split > n) n = p.few_split;
+    if (p.chunk && p.chunk_split > n) n = p.chunk_split;
+    return n > 1 ? (size_t) n * (size_t) rows * (size_t) (hd + 2) * sizeof(float) : 0;
+}
+
+bool attn_args(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new, int64_t max_keys) {
+    return nh >= 1 && nh <= 65535 && kv->n_kv >= 1 && nh % kv->n_kv == 0 && max_new >= 0 && max_keys >= 0
+           && tokens >= 0 && tokens * nh <= INT32_MAX;
 }
 
 }  // namespace
@@ -113,8 +785,10 @@ void launch_attn(const PagedAttn & a, int hd, int nh, bool f32, hipStream_t st) 
 
 extern "C" size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new,
                                                   int64_t max_keys) {
-    (void) kv; (void) tokens; (void) nh; (void) max_new; (void) max_keys;
-    return 0;
+    using namespace gsvk;
+    if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0) return 0;
+    if (kv->hd != 32 && kv->hd != 64 && kv->hd != 128) return 0;
+    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys), tokens * nh, kv->hd);
 }
 
 extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
@@ -126,10 +800,11 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     GSVK_TRY(paged_view(kv, tokens, "attn_paged", a.kv));
     GSVK_REQUIRE(nh >= 1 && nh <= 65535 && nh % kv->n_kv == 0, "attn_paged: nh %d is not a multiple of n_kv %d", nh,
                  kv->n_kv);
+    GSVK_REQUIRE(window >= 0 && max_new >= 0 && max_keys >= 0, "attn_paged: window, max_new and max_keys must not be negative");
+    GSVK_REQUIRE(attn_args(kv, tokens, nh, max_new, max_keys), "attn_paged: tokens * nh must be below 2^31");
     GSVK_REQUIRE(out_type == GSVK_TYPE_F32 || out_type == kv->type,
                  "attn_paged: out_type %d is neither F32 nor the cache's type", out_type);
     GSVK_REQUIRE(scale > 0.0f && std::isfinite(scale * 1.4426950408889634f), "attn_paged: scale must be positive and finite");
-    GSVK_REQUIRE(window >= 0 && max_new >= 0 && max_keys >= 0, "attn_paged: window, max_new and max_keys must not be negative");
     if (tokens == 0 || kv->B == 0 || max_new == 0) return GSVK_OK;
     GSVK_REQUIRE(q && out, "attn_paged: q and out must be given");
     const int64_t w = (int64_t) nh * kv->hd;
@@ -137,7 +812,9 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     GSVK_REQUIRE((((uintptr_t) q | (uintptr_t) out) & 15) == 0 && q_stride % 8 == 0
                      && out_stride % (out_type == GSVK_TYPE_F32 ? 4 : 8) == 0,
                  "attn_paged: the rows of q and out must be 16-byte aligned");
-    const size_t need = gsvk_attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys);
+    const int group = nh / kv->n_kv;
+    const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys);
+    const size_t need = workspace_of(p, tokens * nh, kv->hd);
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
     a.q = (const uint16_t *) q;
@@ -147,11 +824,17 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     a.lse = lse;
     a.prefix = prefix;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.group = nh / kv->n_kv;
+    a.group = group;
     a.window = window;
     a.max_new = max_new < tokens ? max_new : (int) tokens;
-    if (kv->type == GSVK_TYPE_F16) launch_attn<PgF16>(a, kv->hd, nh, out_type == GSVK_TYPE_F32, (hipStream_t) stream);
-    else launch_attn<PgBF16>(a, kv->hd, nh, out_type == GSVK_TYPE_F32, (hipStream_t) stream);
+    a.out_f32 = out_type == GSVK_TYPE_F32;
+    if (need) {
+        const int n = (int) (need / ((size_t) tokens * nh * (kv->hd + 2) * sizeof(float)));
+        a.part_o = (float *) ws;
+        a.part_ml = a.part_o + (size_t) n * tokens * nh * kv->hd;
+    }
+    if (kv->type == GSVK_TYPE_F16) launch_attn<PgF16>(a, kv->hd, p, (hipStream_t) stream);
+    else launch_attn<PgBF16>(a, kv->hd, p, (hipStream_t) stream);
     GSVK_LAUNCH_CHECK();
     return GSVK_OK;
 }

@@ -521,7 +521,8 @@ int gsvk_op_attn_prefill(const float * qkv, int B, int S, int max_len, const int
  *                [seq_start[b], seq_start[b + 1]) of the token arrays (none is allowed). Rows from
  *                seq_start[B] on belong to no sequence: nothing is written for them.
  *  kv_len      : [B] int32: keys of sequence b, its new tokens' among them: row i of its n new
- *                rows is key kv_len[b] - n + i. Keys past table_cols * page_size do not exist. */
+ *                rows is key kv_len[b] - n + i. Keys past table_cols * page_size (or past 2^31 - 256)
+ *                do not exist. */
 typedef struct gsvk_paged_kv {
     void * k;
     void * v;
@@ -580,7 +581,7 @@ int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, const void * 
  * key gives zeros and -inf. What a row does not see has no effect on it, whatever it holds
  * (infinities and NaN too).
  * max_new: the most new tokens of any sequence (rows past it are not computed); max_keys: the most
- * keys of any sequence, which only decides how the work is split. scale > 0.
+ * keys of any sequence, which only decides how the work is split. scale > 0; tokens * nh < 2^31.
  * ws: gsvk_attn_paged_workspace_bytes() bytes of device memory of the same arguments (NULL if 0);
  * nothing in it outlives the call. Results do not depend on what else runs, and are the same bits
  * for the same arguments. */

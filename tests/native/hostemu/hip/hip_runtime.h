@@ -163,6 +163,55 @@ inline C __builtin_amdgcn_mfma_i32_32x32x32_i8(A a, A b, C c, int, int, int) { r
 template <typename A, typename C>
 inline C __builtin_amdgcn_mfma_f32_32x32x16_f16(A a, A b, C c, int, int, int) { return emu_mfma_32x32<_Float16, 8>(a, b, c); }
 
+template <typename A, typename C>
+inline C __builtin_amdgcn_mfma_f32_32x32x16_bf16(A a, A b, C c, int, int, int) { return emu_mfma_32x32<__bf16, 8>(a, b, c); }
+
+// 16 x 16 x 32: lane 16 g + i holds row (A) / column (B) i's K values [8 g, 8 g + 8), and of the result
+// column i of the rows 4 g + v.
+template <typename E, typename A, typename C>
+inline C emu_mfma_16x16(A a, A b, C c) {
+    static E s_a[16][64][8], s_b[16][64][8];
+    static_assert(sizeof(A) == 8 * sizeof(E), "operand size");
+    const int lane = (int) (threadIdx.x & 63), wave = (int) (threadIdx.x >> 6);
+    std::memcpy(s_a[wave][lane], &a, sizeof a);
+    std::memcpy(s_b[wave][lane], &b, sizeof b);
+    ::emu::wave_sync();
+    for (int v = 0; v < 4; v++) {
+        float s = c[v];
+        for (int g = 0; g < 4; g++)
+            for (int k = 0; k < 8; k++)
+                s += (float) s_a[wave][16 * g + 4 * (lane >> 4) + v][k] * (float) s_b[wave][16 * g + (lane & 15)][k];
+        c[v] = s;
+    }
+    ::emu::wave_sync();
+    return c;
+}
+template <typename A, typename C>
+inline C __builtin_amdgcn_mfma_f32_16x16x32_f16(A a, A b, C c, int, int, int) { return emu_mfma_16x16<_Float16>(a, b, c); }
+template <typename A, typename C>
+inline C __builtin_amdgcn_mfma_f32_16x16x32_bf16(A a, A b, C c, int, int, int) { return emu_mfma_16x16<__bf16>(a, b, c); }
+
+// ---- transposing LDS read: of each 16 lanes, lane 4 j + c points at columns 4 c .. 4 c + 3 of row j,
+// lane i receives column i of the four rows ----
+typedef short emu_s4 __attribute__((ext_vector_type(4)));
+inline emu_s4 __builtin_amdgcn_ds_read_tr16_b64_v4i16(__attribute__((address_space(3))) emu_s4 * p) {
+    uint64_t own;
+    std::memcpy(&own, (const char *) p, 8);
+    const int lane = (int) (threadIdx.x & 63), i = lane & 15;
+    emu_s4 r;
+    for (int j = 0; j < 4; j++)
+        r[j] = (short) (::emu::shfl(own, (lane & ~15) + 4 * j + i / 4, 64) >> (16 * (i & 3)));
+    return r;
+}
+
+// the upper half of the first operand and the lower half of the second change places
+struct emu_u2 { unsigned v[2]; unsigned operator[](int i) const { return v[i]; } };
+inline emu_u2 __builtin_amdgcn_permlane32_swap(unsigned a, unsigned b, bool, bool) {
+    const int lane = (int) (threadIdx.x & 63);
+    const unsigned bl = ::emu::shfl(b, lane & 31, 64), ah = ::emu::shfl(a, (lane & 31) + 32, 64);
+    return lane < 32 ? emu_u2{{a, ah}} : emu_u2{{bl, b}};
+}
+
 // ---- direct global -> LDS loads: lane L's bytes to lds + L * size, at once (a wait that is missing
 // is not seen here) ----
 inline void __builtin_amdgcn_global_load_lds(const void * g, __attribute__((address_space(3))) void * lds, int size, int, int) {

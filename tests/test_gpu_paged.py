@@ -486,6 +486,9 @@ def test_another_stream(gpu):
     for bt, kv, q, out, ws, st in sets:
         ref, _, dout, _ = bt.attn(scale)
         assert np.all(np.abs(out.cpu().double().numpy() - ref) <= dout + rounding(np.abs(ref) + dout, "bf16"))
+    bt, kv, q, out, ws, st = sets[0]
+    with pytest.raises(ValueError):      # a workspace of torch's current stream on another one
+        gpu.op_attn_paged(kv, q, scale, out, max_new=3, max_keys=4000, stream=st.cuda_stream)
 
 
 def test_wrong_tensors_are_refused(gpu):

@@ -76,3 +76,22 @@ def test_nothing_to_do_is_no_error():
     """No tokens or no sequences: nothing is launched (there is no device here)."""
     assert _append(_kv(), tokens=0) == 0 and _append(_kv(B=0)) == 0
     assert _attn(_kv(), tokens=0) == 0 and _attn(_kv(B=0)) == 0 and _attn(_kv(), max_new=0) == 0
+
+
+def _ws(kv, tokens, nh, max_new, max_keys):
+    return gsvk.lib().gsvk_attn_paged_workspace_bytes(C.byref(kv), tokens, nh, max_new, max_keys)
+
+
+def test_workspace_is_asked_for():
+    """One long sequence is split over its keys: a call without the workspace it needs is refused; one
+    short sequence needs none."""
+    kv = _kv(table_stride=10000, table_cols=10000, n_pages=10000, B=1)
+    need = _ws(kv, 1, 4, 1, 100000)
+    assert need > 0
+    assert _attn(kv, tokens=1, max_new=1, max_keys=100000) == 1
+    assert "workspace" in gsvk.last_error()
+    assert _attn(kv, tokens=1, max_new=1, max_keys=100000, ws=4096, ws_bytes=need - 1) == 1
+    assert _attn(kv, tokens=1, max_new=1, max_keys=100000, ws=4104, ws_bytes=need) == 1
+    assert _ws(kv, 1, 4, 1, 16) == 0
+    assert _ws(_kv(hd=48), 1, 4, 1, 100000) == 0      # (arguments that the call itself refuses)
+    assert gsvk.lib().gsvk_attn_paged_workspace_bytes(None, 1, 4, 1, 100000) == 0
