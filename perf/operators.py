@@ -202,12 +202,19 @@ def prepare(case, seed):
 
 # ---- one call -----------------------------------------------------------------------------
 
+_module = None
+
+
 def _gsvk():
-    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gsv.cpp_amd")
-    if package not in sys.path:
-        sys.path.insert(0, package)
-    import gsvk
-    return gsvk
+    """The framework's Python binding, found once."""
+    global _module
+    if _module is None:
+        package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gsv.cpp_amd")
+        if package not in sys.path:
+            sys.path.insert(0, package)
+        import gsvk
+        _module = gsvk
+    return _module
 
 
 def _split(s):
