@@ -31,7 +31,8 @@
 // What a row does not see must not reach it. Scores of unseen keys are replaced by -inf. Values
 // of keys that no row of the tile sees are replaced by zeros on their way to LDS. Where some rows
 // of a tile see a key and others do not, 0 * inf would still give NaN: such blocks are searched
-// for infinities and NaNs, which are taken out of the product and added one by one (rare).
+// for infinities and NaNs, which are taken out of the product and added to the rows that see them
+// (rare; a positive probability times an infinity is that infinity).
 #include <cfloat>
 #include <cmath>
 
@@ -44,6 +45,7 @@ typedef float pg_f4 __attribute__((ext_vector_type(4)));
 typedef float pg_f16 __attribute__((ext_vector_type(16)));
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pg_s4 pg_lds4;
+typedef __attribute__((address_space(3))) uint16_t pg_lds1;
 
 constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
 constexpr int FEW_WAVES = 4, FEW_KEYS = 32;
@@ -104,11 +106,13 @@ __device__ __forceinline__ float sum_x32(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Swizzles of 16-byte pieces inside a key's LDS row of HD values, so that the rows that one read
-// touches fall in different banks (256 bytes): for V pairs of pieces (the transposing read takes 32
-// bytes of 4 keys), for K single ones (16 bytes of 16 keys).
+// Swizzles of 16-byte pieces inside a key's LDS row of HD values, so that what 32 lanes read falls in
+// different banks (256 bytes): for K 16 bytes of 16 keys, for V (read transposed) 32 bytes of 8 keys
+// with the 16-row products, 64 bytes of 4 keys with the 32-row ones.
 template <int HD>
 __device__ __forceinline__ int swz_v(int key) { return 2 * ((key / (128 / HD)) & (HD / 16 - 1)); }
+template <int HD>
+__device__ __forceinline__ int swz_vc(int key) { return 4 * ((key / (128 / HD)) & (HD / 32 - 1)); }
 template <int HD>
 __device__ __forceinline__ int swz_k(int key) { return (key / (128 / HD)) & (HD / 8 - 1); }
 
@@ -343,7 +347,6 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
             for (int v = 0; v < 8; v++) {
                 p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][v >> 2][v & 3], a.scale_log2, -m[t]));
                 sum += p[v];
-                sc[t][v >> 2][v & 3] = p[v];
             }
             l[t] += sum;
             pf[t] = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
@@ -366,17 +369,13 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
                 const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lg;
 #pragma unroll
                 for (int t = 0; t < QT; t++) {
-                    float mine = 0.0f;
-#pragma unroll
-                    for (int v = 0; v < 8; v++) mine = (j >> 4) * 4 + (j & 3) == v ? sc[t][v >> 2][v & 3] : mine;
-                    const float p = __shfl(mine, li + 16 * ((j & 15) >> 2), 64);
                     const bool see = key >= lo[t] && key < hi[t];
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const uint16_t u = vp[16 * d + e];
-                            if (see && is_odd<T>(u)) o[t][d][e] += p * T::up(u);
+                            if (see && is_odd<T>(u)) o[t][d][e] += T::up(u);
                         }
                 }
             }
@@ -440,13 +439,34 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
 
 // ---- chunks ----------------------------------------------------------------------------------------
 
+// A wave's direct load of 1 KB: lane L's 16 bytes at base + off (bytes) to lds + 16 L. In asm, since the
+// compiler waits for every direct load in flight before any LDS read that it cannot tell apart
+// from their targets (and the tile after this one is in flight while this one is read). No outputs;
+// the waits are wait_loads'. The s_nop is the wait state between a write of m0 and a load that reads it.
+__device__ __forceinline__ void load_lds(const char * base, uint32_t off, uint16_t * lds) {
+#ifdef GSVK_HOSTEMU
+    __builtin_amdgcn_global_load_lds(base + off, (pg_lds1 *) lds, 16, 0, 0);
+#else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"((uint32_t) (uintptr_t) (pg_lds1 *) lds), "v"(off), "s"(base)
+                 : "memory");
+#endif
+}
+// every load of this wave has landed, every LDS operation of it is done; then all waves' are
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt(0x7 << 4);   // gfx9: vmcnt 0, lgkmcnt 0, expcnt not waited on
+    __syncthreads();
+}
+
 template <class T, int HD>
 __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn a) {
-    constexpr int C = HD / 8, NT = CH_WAVES * 64, UNITS = CH_KEYS * C, NU = 2 * UNITS / NT;
+    constexpr int C = HD / 8, NT = CH_WAVES * 64;
     constexpr int NK = HD / 16, DT = HD / 32;
+    constexpr int NL = C >= CH_WAVES ? C / CH_WAVES : 1;   // direct loads of a wave per tile of K (and of V)
     __shared__ __align__(16) uint16_t s_k[2][CH_KEYS * HD];
     __shared__ __align__(16) uint16_t s_v[2][CH_KEYS * HD];
-    __shared__ int s_odd[2];
+    __shared__ int s_flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
 
     const int b = blockIdx.z, kvh = blockIdx.y;
     const int split = blockIdx.x % a.nsplit;
@@ -457,14 +477,15 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
     const int r0 = rt * CH_WAVES * 32;
     if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
     const int nh = a.group * a.kv.n_kv;
-    // the key range of the workgroup and of this wave
+    // the key ranges of the workgroup and of this wave
     const int tokf = r0 / a.group, tokl = (min(r0 + CH_WAVES * 32, s.rows) - 1) / a.group;
     const int klo = key_lo(a, s, tokf), khi = key_hi(s, tokl);
-    const bool ragged = key_lo(a, s, tokl) > klo || key_hi(s, tokf) < khi;
+    const int lo_max = key_lo(a, s, tokl), hi_min = key_hi(s, tokf);
     const int rw = r0 + wave * 32;
     const bool idle = rw >= s.rows;
     const int tw0 = min(rw, s.rows - 1) / a.group, tw1 = min(rw + 31, s.rows - 1) / a.group;
-    const int wlo = key_lo(a, s, tw0), wlo_max = key_lo(a, s, tw1), whi_min = key_hi(s, tw0), whi = key_hi(s, tw1);
+    const int wlo = key_lo(a, s, tw0), wlo_max = key_lo(a, s, tw1), whi_min = key_hi(s, tw0);
+    const int whi = idle ? 0 : key_hi(s, tw1);
     const int r = min(rw + li, s.rows - 1), tok = r / a.group, h = kvh * a.group + r % a.group;
     const int lo = key_lo(a, s, tok), hi = key_hi(s, tok);
 
@@ -477,98 +498,134 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
     const int kt_a = klo / CH_KEYS, nkt = khi > klo ? (khi + CH_KEYS - 1) / CH_KEYS - kt_a : 0;
     const int per = (nkt + a.nsplit - 1) / a.nsplit;
     const int kt0 = kt_a + min(nkt, split * per), kt1 = kt_a + min(nkt, (split + 1) * per);
-
     const int32_t * tb = a.kv.table + b * a.kv.table_stride;
-    // pages of a tile's four groups of 16 keys
-    struct Pages { int p[CH_KEYS / 16]; };
-    const auto pages = [&](int kt) {
-        Pages g;
+
+    // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (8 j + wave) * 64 on
+    // (all within one group of 16 keys, one page); with 32 dims waves 0-3 load K, 4-7 V.
+    uint32_t off_k[NL], off_v[NL];
 #pragma unroll
-        for (int i = 0; i < CH_KEYS / 16; i++) g.p[i] = page_of(a, tb, kt * CH_KEYS + 16 * i);
-        return g;
-    };
-    // A thread's 16-byte units of a tile: K first, then V, in the order of the keys; the 64 units of a
-    // wave lie in one group of 16 keys.
-    uint4 st[NU];
-    const auto fetch = [&](int kt, const Pages & g) {
+    for (int j = 0; j < NL; j++) {
+        const int u = ((j * CH_WAVES + wave) % C) * 64 + lane, key = u / C;
+        off_k[j] = ((key & 15) * HD + (((u % C) ^ swz_k<HD>(key)) << 3)) * 2;
+        off_v[j] = ((key & 15) * HD + (((u % C) ^ swz_vc<HD>(key)) << 3)) * 2;
+    }
+    int64_t at_v[NL] = {};   // byte offsets of the wave's key groups in the tile whose V comes next
+    const auto offsets = [&](int kt, int64_t (&at)[NL]) {
 #pragma unroll
-        for (int i = 0; i < NU; i++) {
-            const int w0 = i * NT + wave * 64, uu = w0 % UNITS, kg = uu / C / 16;
-            const int pg = kg == 0 ? g.p[0] : kg == 1 ? g.p[1] : kg == 2 ? g.p[2] : g.p[3];
-            const int64_t at = key_at<HD>(a, pg, kvh, kt * CH_KEYS + 16 * kg) + (uu - kg * 16 * C) * 8;
-            st[i] = *reinterpret_cast<const uint4 *>((w0 < UNITS ? a.kv.k : a.kv.v) + at + lane * 8);
+        for (int j = 0; j < NL; j++) {
+            const int key = kt * CH_KEYS + ((j * CH_WAVES + wave) % C) * (CH_KEYS / C) / 16 * 16;
+            at[j] = key_at<HD>(a, page_of(a, tb, key), kvh, key) * 2;
         }
     };
-    const auto stage = [&](int kt, const Pages & g, int buf) {
+    const auto load = [&](const uint16_t * cache, const int64_t (&at)[NL], const uint32_t (&off)[NL], uint16_t * lds) {
 #pragma unroll
-        for (int i = 0; i < NU; i++) {
-            const int w0 = i * NT + wave * 64, uu = w0 % UNITS, kg = uu / C / 16;
-            const int u = uu + lane, key = u / C;
-            if (w0 < UNITS) {
-                *reinterpret_cast<uint4 *>(&s_k[buf][key * HD + (((u % C) ^ swz_k<HD>(key)) << 3)]) = st[i];
-            } else {
-                const int pg = kg == 0 ? g.p[0] : kg == 1 ? g.p[1] : kg == 2 ? g.p[2] : g.p[3];
-                const int at = kt * CH_KEYS + key;
-                if (!(pg >= 0 && at >= klo && at < khi)) st[i] = make_uint4(0, 0, 0, 0);
-                if (ragged && any_odd<T>(st[i])) {
-                    clear_odd<T>(st[i]);
-                    s_odd[buf] = kt + 1;
-                }
-                *reinterpret_cast<uint4 *>(&s_v[buf][key * HD + (((u % C) ^ swz_v<HD>(key)) << 3)]) = st[i];
-            }
-        }
+        for (int j = 0; j < NL; j++)
+            load_lds(reinterpret_cast<const char *>(cache) + at[j], off[j], lds + ((j * CH_WAVES + wave) % C) * 512);
+    };
+    const auto load_k = [&](const int64_t (&at)[NL], int buf) {
+        if (HD > 32 || wave < 4) load(a.kv.k, at, off_k, s_k[buf]);
+    };
+    const auto load_v = [&](const int64_t (&at)[NL], int buf) {
+        if (HD > 32 || wave >= 4) load(a.kv.v, at, off_v, s_v[buf]);
     };
 
     float m = M_NONE, l = 0.0f;
     pg_f16 o[DT];
 #pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) o[d][v] = 0.0f;
+    for (int d = 0; d < DT; d++) o[d] = pg_f16{};
 
-    if (tid < 2) s_odd[tid] = 0;
-    __syncthreads();
-    Pages cur{}, nxt{};
-    if (kt0 < kt1) {
-        cur = pages(kt0);
-        fetch(kt0, cur);
-        stage(kt0, cur, 0);
-        nxt = pages(min(kt0 + 1, kt1 - 1));
-    }
-    __syncthreads();
-    int buf = 0;
-    for (int kt = kt0; kt < kt1; kt++, buf ^= 1) {
-        const bool more = kt + 1 < kt1;
-        if (more) fetch(kt + 1, nxt);
-        const Pages nn = pages(min(kt + 2, kt1 - 1));
+    // operand registers: K of a quarter of the scores' products (k = q / 2), V of the 16 keys 16 q .. + 15
+    const auto read_k = [&](uint4 (&kf)[NK / 2], int buf, int q) {
+        const int key = 32 * (q >> 1) + li;
+#pragma unroll
+        for (int i = 0; i < NK / 2; i++) {
+            const int c = (q & 1) * (NK / 2) + i;
+            kf[i] = *reinterpret_cast<const uint4 *>(&s_k[buf][key * HD + (((2 * c + lh) ^ swz_k<HD>(key)) << 3)]);
+        }
+    };
+    const auto read_v = [&](typename T::v8 (&vf)[DT], int buf, int q) {
+        const int key = 16 * q + 4 * lh + ((lane & 15) >> 2);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            const uint16_t * p = &s_v[buf][key * HD + ((ch ^ swz_vc<HD>(key)) << 3) + 4 * (lane & 1)];
+            const uint16_t * p2 = &s_v[buf][(key + 8) * HD + ((ch ^ swz_vc<HD>(key + 8)) << 3) + 4 * (lane & 1)];
+            vf[d] = v8_of<T>(lds_tr4(p), lds_tr4(p2));
+        }
+    };
+    const auto mul_k = [&](pg_f16 (&sc)[2], const uint4 (&kf)[NK / 2], int q) {
+#pragma unroll
+        for (int i = 0; i < NK / 2; i++) {
+            const int c = (q & 1) * (NK / 2) + i;
+            sc[q >> 1] = mfma32<T>(v8_of<T>(kf[i]), qf[c], c ? sc[q >> 1] : pg_f16{});
+        }
+    };
+    // S^T of the tile in buffer buf
+    const auto scores = [&](pg_f16 (&sc)[2], int buf) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            uint4 kf[NK / 2];
+            read_k(kf, buf, q);
+            mul_k(sc, kf, q);
+        }
+    };
+    bool has_bad = false;
+    // unseen keys of tile kt to -inf
+    const auto mask = [&](pg_f16 (&sc)[2], int kt) {
         const int kb = kt * CH_KEYS;
-        const bool okp = cur.p[0] >= 0 && cur.p[1] >= 0 && cur.p[2] >= 0 && cur.p[3] >= 0;
-        if (!idle && kb < whi && kb + CH_KEYS > wlo) {
-            const bool full = kb >= wlo_max && kb + CH_KEYS <= whi_min && okp;
-            pg_f16 sc[2];
+        uint32_t ok = 0xf;
+        if (has_bad) {
+            ok = 0;
+            for (int g = 0; g < CH_KEYS / 16; g++) ok |= (uint32_t) (page_of(a, tb, kb + 16 * g) >= 0) << g;
+        }
+        const int from = lo - kb - 4 * lh;
+        const uint32_t num = (uint32_t) max(hi - lo, 0);
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) sc[k][v] = 0.0f;
-                const int key = 32 * k + li;
+            for (int v = 0; v < 16; v++) {
+                const int j = 32 * k + 8 * (v >> 2) + (v & 3);   // (+ 4 lh)
+                if ((uint32_t) (j - from) >= num) sc[k][v] = -INFINITY;
+                if ((v & 7) == 7) {
+                    if (!((ok >> (2 * k + (v >> 3))) & 1))
 #pragma unroll
-                for (int c = 0; c < NK; c++) {
-                    const uint4 kf = *reinterpret_cast<const uint4 *>(&s_k[buf][key * HD + (((2 * c + lh) ^ swz_k<HD>(key)) << 3)]);
-                    sc[k] = mfma32<T>(v8_of<T>(kf), qf[c], sc[k]);
+                        for (int w = v - 7; w <= v; w++) sc[k][w] = -INFINITY;
+                    __builtin_amdgcn_sched_barrier(0);   // (otherwise all 32 conditions are held at once)
                 }
             }
-            if (!full) {
+    };
+    const auto top_of = [&](const pg_f16 (&sc)[2]) {
+        float top = fmaxf(sc[0][0], sc[1][0]);
 #pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int v = 0; v < 16; v++) {
-                        const int j = 32 * k + 8 * (v >> 2) + 4 * lh + (v & 3);
-                        if (!(kb + j >= lo && kb + j < hi && cur.p[2 * k + (v >> 3)] >= 0)) sc[k][v] = -INFINITY;
-                    }
+        for (int v = 1; v < 16; v++) top = fmaxf(fmaxf(top, sc[0][v]), sc[1][v]);
+        return top;
+    };
+    float top = -INFINITY;   // this lane's largest score of the current tile
+    // Tile kt: S^T in sc, V in buffer buf; computes S^T of the tile after it from the other buffer.
+    // In four stages of 16 keys: a stage's exponentials run while the matrix cores work on a
+    // quarter of the next scores and on the weighted sum of the stage before.
+    const auto step = [&](int kt, pg_f16 (&sc)[2], pg_f16 (&sn)[2], int buf) {
+        const int kb = kt * CH_KEYS;
+        if (kb < lo_max || kb + CH_KEYS > hi_min || has_bad) {
+            // values that no row sees become zeros; infinities and NaNs are taken out
+            for (int u = tid; u < CH_KEYS * C; u += NT) {
+                const int key = u / C;
+                uint4 * p = reinterpret_cast<uint4 *>(&s_v[buf][u * 8]);
+                uint4 x = *p;
+                const bool see = kb + key >= klo && kb + key < khi && (!has_bad || page_of(a, tb, kb + key) >= 0);
+                if (see && !any_odd<T>(x)) continue;
+                if (see) s_flag[1] = kt + 1;
+                clear_odd<T>(x);
+                *p = see ? x : make_uint4(0, 0, 0, 0);
             }
-            float top = fmaxf(sc[0][0], sc[1][0]);
-#pragma unroll
-            for (int v = 1; v < 16; v++) top = fmaxf(fmaxf(top, sc[0][v]), sc[1][v]);
+            __syncthreads();
+        }
+        if (kt + 1 < kt1) load_v(at_v, buf ^ 1);
+        if (kt + 2 < kt1) {
+            offsets(kt + 2, at_v);
+            load_k(at_v, buf);
+        }
+        if (kb < whi && kb + 2 * CH_KEYS > wlo) {   // a row of the wave sees this tile, or the next one
             top *= a.scale_log2;
             if (__any(top > m + M_ROOM)) {
                 const float mn = fmaxf(m, max_x32(top) - M_SET);
@@ -580,57 +637,84 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[d][v] *= f;
             }
-            float sum = 0.0f;
+            uint4 kf[2][NK / 2];
+            typename T::v8 vf[2][DT], pf;
+            read_k(kf[0], buf ^ 1, 0);
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int q = 0; q < 4; q++) {
+                if (q < 3) read_k(kf[(q + 1) & 1], buf ^ 1, q + 1);
+                read_v(vf[q & 1], buf, q);
+                mul_k(sn, kf[q & 1], q);
+                if (q > 0) {
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    sc[k][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[k][v], a.scale_log2, -m));
-                    sum += sc[k][v];
+                    for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[(q - 1) & 1][d], pf, o[d]);
                 }
-            l += sum;
+                float p[8], sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    const int v0 = 8 * c;
-                    const typename T::v8 pf = v8_of<T>(make_uint4(
-                        pg_pack<T>(sc[k][v0], sc[k][v0 + 1]), pg_pack<T>(sc[k][v0 + 2], sc[k][v0 + 3]),
-                        pg_pack<T>(sc[k][v0 + 4], sc[k][v0 + 5]), pg_pack<T>(sc[k][v0 + 6], sc[k][v0 + 7])));
-                    const int key = 32 * k + 16 * c + 4 * lh + ((lane & 15) >> 2);
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                        const uint16_t * p = &s_v[buf][key * HD + ((ch ^ swz_v<HD>(key)) << 3) + 4 * (lane & 1)];
-                        const uint16_t * p2 = &s_v[buf][(key + 8) * HD + ((ch ^ swz_v<HD>(key + 8)) << 3) + 4 * (lane & 1)];
-                        o[d] = mfma32<T>(v8_of<T>(lds_tr4(p), lds_tr4(p2)), pf, o[d]);
-                    }
+                for (int v = 0; v < 8; v++) {
+                    p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[q >> 1][8 * (q & 1) + v], a.scale_log2, -m));
+                    sum += p[v];
                 }
-            if (s_odd[buf] == kt + 1) {   // the infinities and NaNs that some of the rows see
+                l += sum;
+                asm volatile("" : "+v"(l));   // (summed here: put off, the sum would keep all 32 values live)
+                pf = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
+                                         pg_pack<T>(p[6], p[7])));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[1][d], pf, o[d]);
+            if (s_flag[1] == kt + 1) {   // the infinities and NaNs that some of the rows see
                 for (int j = 0; j < CH_KEYS; j++) {
                     const int key = kb + j, page = page_of(a, tb, key);
                     if (page < 0 || key < klo || key >= khi) continue;
                     const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lh;
-                    float mine = 0.0f;
-#pragma unroll
-                    for (int v = 0; v < 32; v++)
-                        mine = (j >> 5) * 16 + ((j >> 3) & 3) * 4 + (j & 3) == v ? sc[v >> 4][v & 15] : mine;
-                    const float p = __shfl(mine, li + 32 * ((j >> 2) & 1), 64);
                     const bool see = key >= lo && key < hi;
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
                         for (int v = 0; v < 16; v++) {
                             const uint16_t u = vp[32 * d + 8 * (v >> 2) + (v & 3)];
-                            if (see && is_odd<T>(u)) o[d][v] += p * T::up(u);
+                            if (see && is_odd<T>(u)) o[d][v] += T::up(u);
+                            if ((v & 3) == 3) __builtin_amdgcn_sched_barrier(0);
                         }
                 }
             }
+            if (!(kb + CH_KEYS >= wlo_max && kb + 2 * CH_KEYS <= whi_min && !has_bad)) mask(sn, kt + 1);
+            top = top_of(sn);
         }
-        if (more) stage(kt + 1, nxt, buf ^ 1);
-        cur = nxt;
-        nxt = nn;
+        wait_loads();
+    };
+
+    if (kt0 < kt1) {
+        if (tid < 2) s_flag[tid] = 0;
         __syncthreads();
+        // table entries that name no page: rare, and every tile then takes its masks
+        const int c0 = (kt0 * CH_KEYS) >> a.kv.page_shift, c1 = (min(kt1 * CH_KEYS, khi) - 1) >> a.kv.page_shift;
+        for (int c = c0 + tid; c <= c1; c += NT)
+            if (page_of(a, tb, c << a.kv.page_shift) < 0) s_flag[0] = 1;
+        int64_t at[NL];
+        offsets(kt0, at);
+        load_k(at, 0);
+        load_v(at, 0);
+        offsets(min(kt0 + 1, kt1 - 1), at_v);
+        load_k(at_v, 1);
+        wait_loads();
+        has_bad = __builtin_amdgcn_readfirstlane(s_flag[0]) != 0;
+        // (a wave whose rows see none of the first tiles passes over them: its scores are then these)
+        pg_f16 s0[2], s1[2];
+#pragma unroll
+        for (int v = 0; v < 16; v++) s1[0][v] = s1[1][v] = -INFINITY;
+        scores(s0, 0);
+        {
+            const int kb = kt0 * CH_KEYS;
+            if (!(kb >= wlo_max && kb + CH_KEYS <= whi_min && !has_bad)) mask(s0, kt0);
+            top = top_of(s0);
+        }
+        __syncthreads();   // (buffer 0 of K is free)
+        for (int kt = kt0; kt < kt1; kt += 2) {
+            step(kt, s0, s1, 0);
+            if (kt + 1 < kt1) step(kt + 1, s1, s0, 1);
+        }
     }
 
     if (idle) return;

@@ -355,31 +355,48 @@ def op_qkv_attn(wq, wd, bias, res, r, ln_bias, wb, k, v, kv_begin, col, scale, o
 
 def _gsvk_type(dtype):
     """GGML type number of a torch dtype (F32, F16 or BF16)."""
-    name = str(dtype)
-    try:
-        return {"torch.float32": GSVK_TYPE_F32, "torch.float16": GSVK_TYPE_F16, "torch.bfloat16": GSVK_TYPE_BF16}[name]
-    except KeyError:
-        raise ValueError(f"gsvk: {name} is not a type of the paged-cache operators") from None
+    t = _TYPES.get(dtype)
+    if t is None:
+        import torch
+        _TYPES.update({torch.float32: GSVK_TYPE_F32, torch.float16: GSVK_TYPE_F16, torch.bfloat16: GSVK_TYPE_BF16})
+        t = _TYPES.get(dtype)
+        if t is None:
+            raise ValueError(f"gsvk: {dtype} is not a type of the paged-cache operators")
+    return t
+
+
+_TYPES = {}
 
 
 def _rows_of(t, what, width, device):
-    """Row stride of a token array [T][width] or [T][heads][hd] whose rows are contiguous."""
-    inner = 1
-    for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if n != 1 and st != inner:
-            raise ValueError(f"{what}: the rows must be contiguous")
-        inner *= n
-    if t.dim() < 2 or inner != width:
-        raise ValueError(f"{what}: rows of {width} elements expected")
-    if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, the cache on {device}")
-    return t.stride(0) if t.shape[0] > 1 else inner
+    """Row stride of a token array [T][width] or [T][heads][hd] on device number `device` whose rows
+    are contiguous."""
+    sh, st = t.shape, t.stride()
+    if len(sh) == 2:
+        ok = sh[1] == width and st[1] == 1
+    else:
+        ok = len(sh) == 3 and sh[1] * sh[2] == width and st[2] == 1 and (st[1] == sh[2] or sh[1] == 1)
+    if not ok:
+        raise ValueError(f"{what}: contiguous rows of {width} elements expected, got {list(sh)} with strides {list(st)}")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: on {t.device}, the cache on device {device}")
+    return st[0] if sh[0] > 1 else width
 
 
 def _int32(t, what, shape, device):
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{what}: a contiguous int32 tensor of shape {list(shape)} on {device} expected")
-    return t
+    if _int32_ok(t, shape, device):
+        return t.data_ptr()
+    raise ValueError(f"{what}: a contiguous int32 tensor of shape {list(shape)} on device {device} expected")
+
+
+def _int32_ok(t, shape, device):
+    return t.element_size() == 4 and not t.is_floating_point() and not t.is_complex() and t.shape == shape \
+        and t.is_contiguous() and t.get_device() == device
+
+
+def _f32_ok(t, shape, device):
+    return t.element_size() == 4 and t.is_floating_point() and t.shape == shape and t.is_contiguous() \
+        and t.get_device() == device
 
 
 class PagedKV:
@@ -395,14 +412,15 @@ class PagedKV:
         inner = (page * hd, hd, 1)
         if any(n != 1 and st != want for n, st, want in zip(k.shape[1:], k.stride()[1:], inner)):
             raise ValueError("PagedKV: a page must be contiguous")
-        if not k.is_cuda or any(t.device != k.device for t in (v, table, seq_start, kv_len)):
+        dev = k.get_device()
+        if not k.is_cuda or any(t.get_device() != dev for t in (v, table, seq_start, kv_len)):
             raise ValueError("PagedKV: every tensor must be on the cache's device")
         if table.dim() != 2 or str(table.dtype) != "torch.int32" or (table.shape[1] != 1 and table.stride(1) != 1):
             raise ValueError("PagedKV: table must be [B][cols] int32 with contiguous rows")
         B, cols = table.shape
-        _int32(seq_start, "PagedKV: seq_start", (B + 1,), k.device)
-        _int32(kv_len, "PagedKV: kv_len", (B,), k.device)
-        self.dtype, self.device, self.type = k.dtype, k.device, _gsvk_type(k.dtype)
+        _int32(seq_start, "PagedKV: seq_start", (B + 1,), dev)
+        _int32(kv_len, "PagedKV: kv_len", (B,), dev)
+        self.dtype, self.device, self.type = k.dtype, dev, _gsvk_type(k.dtype)
         self.n_kv, self.page_size, self.hd, self.B, self.cols = n_kv, page, hd, B, cols
         self.keep = (k, v, table, seq_start, kv_len)
         self.args = PagedKVArgs(k.data_ptr(), v.data_ptr(), self.type, n_kv, hd, page, n_pages,
@@ -410,45 +428,53 @@ class PagedKV:
                                 table.stride(0) if B > 1 else cols, cols, B, seq_start.data_ptr(), kv_len.data_ptr())
         self._ref = C.byref(self.args)
 
-    def _on_device(self, what):
-        import torch
-        if torch.cuda.current_device() != self.device.index:
-            raise ValueError(f"{what}: the cache is on {self.device}, which is not the current device")
+
+def _paged_stream(kv, stream, what):
+    """The stream of a call (torch's current one by default), on the cache's device."""
+    import torch
+    if torch.cuda.current_device() != kv.device:
+        raise ValueError(f"{what}: the cache is on device {kv.device}, which is not the current one")
+    return _raw_stream(kv.device) if stream is None else stream
+
+
+def _raw_stream(device):
+    """Handle of torch's current stream on device number `device`."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the stream object costs 3 us more)
+    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=False, pos=None, n_bad=None,
                     stream=None):
     """Append k, v [T][n_kv * hd] to the pages of `kv` (PagedKV) and rotate q [T][nh * hd] into q_out
     [T][nh][hd] (include/gsvk.h gsvk_op_paged_append); cos, sin [positions][rot / 2] fp32."""
-    kv._on_device("paged_append")
-    T, w = k.shape[0], kv.n_kv * kv.hd
-    if v.shape[0] != T or k.dtype != v.dtype or (q is None) != (q_out is None):
+    dev, st = kv.device, _paged_stream(kv, stream, "paged_append")
+    T, w, x = k.shape[0], kv.n_kv * kv.hd, k.dtype
+    if v.shape[0] != T or v.dtype != x or (q is None) != (q_out is None):
         raise ValueError("paged_append: k and v of the same rows and type, q and q_out together")
-    ks, vs = _rows_of(k, "paged_append: k", w, kv.device), _rows_of(v, "paged_append: v", w, kv.device)
-    nh = qs = 0
+    ks, vs = _rows_of(k, "paged_append: k", w, dev), _rows_of(v, "paged_append: v", w, dev)
+    nh, qs, qp, op = 0, 0, None, None
     if q is not None:
-        if q_out.dim() != 3 or q_out.shape[0] != T or q_out.shape[2] != kv.hd or not q_out.is_contiguous() \
-                or q_out.dtype != kv.dtype or q_out.device != kv.device or q.shape[0] != T or q.dtype != k.dtype:
+        sh = q_out.shape
+        if len(sh) != 3 or sh[0] != T or sh[2] != kv.hd or not q_out.is_contiguous() or q_out.dtype != kv.dtype \
+                or q_out.get_device() != dev or q.shape[0] != T or q.dtype != x:
             raise ValueError("paged_append: q_out must be a dense [T][nh][hd] of the cache's type, q of k's type")
-        nh = q_out.shape[1]
-        qs = _rows_of(q, "paged_append: q", nh * kv.hd, kv.device)
+        nh = sh[1]
+        qs = _rows_of(q, "paged_append: q", nh * kv.hd, dev)
+        qp, op = q.data_ptr(), q_out.data_ptr()
     rope = None
     if cos is not None:
-        if sin is None or cos.dim() != 2 or cos.shape != sin.shape or not cos.is_contiguous() \
-                or not sin.is_contiguous() or str(cos.dtype) != "torch.float32" or cos.dtype != sin.dtype \
-                or cos.device != kv.device or sin.device != kv.device:
+        sh = cos.shape
+        if sin is None or len(sh) != 2 or not _f32_ok(cos, sh, dev) or not _f32_ok(sin, sh, dev):
             raise ValueError("paged_append: cos and sin must be [positions][rot / 2] fp32 alike")
-        if pos is not None:
-            _int32(pos, "paged_append: pos", (T,), kv.device)
-        rope = RopeArgs(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], 1 if pairs else 0,
-                        None if pos is None else pos.data_ptr())
+        rope = C.byref(RopeArgs(cos.data_ptr(), sin.data_ptr(), sh[0], 2 * sh[1], 1 if pairs else 0,
+                                None if pos is None else _int32(pos, "paged_append: pos", (T,), dev)))
     elif sin is not None or pos is not None:
         raise ValueError("paged_append: sin and pos go with cos")
-    if n_bad is not None:
-        _int32(n_bad, "paged_append: n_bad", (1,), kv.device)
-    check(lib().gsvk_op_paged_append(kv._ref, _p(q), _p(k), _p(v), _gsvk_type(k.dtype), T, nh, qs, ks, vs,
-                                     None if rope is None else C.byref(rope), _p(q_out), _p(n_bad),
-                                     _stream(stream)), "paged_append")
+    rc = lib().gsvk_op_paged_append(kv._ref, qp, k.data_ptr(), v.data_ptr(), _gsvk_type(x), T, nh, qs, ks, vs, rope, op,
+                                    None if n_bad is None else _int32(n_bad, "paged_append: n_bad", (1,), dev), st)
+    if rc:
+        check(rc, "paged_append")
 
 
 def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys) -> int:
@@ -459,31 +485,36 @@ def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0,
     """Attention of the new tokens q [T][nh][hd] over the pages of `kv` (PagedKV) into out [T][nh][hd]
     (include/gsvk.h gsvk_op_attn_paged); lse [T][nh] fp32, prefix [B] int32. ws None: a workspace from
     torch's allocator, which belongs to torch's current stream."""
-    kv._on_device("attn_paged")
-    T, nh = q.shape[0], q.shape[1]
-    if q.dim() != 3 or out.shape != q.shape or q.dtype != kv.dtype:
+    dev, st = kv.device, _paged_stream(kv, stream, "attn_paged")
+    sh = q.shape
+    if len(sh) != 3 or out.shape != sh or q.dtype != kv.dtype:
         raise ValueError("attn_paged: q of the cache's type and out must be [T][nh][hd]")
+    T, nh = sh[0], sh[1]
     w = nh * kv.hd
-    qs, os_ = _rows_of(q, "attn_paged: q", w, kv.device), _rows_of(out, "attn_paged: out", w, kv.device)
-    if lse is not None and (tuple(lse.shape) != (T, nh) or str(lse.dtype) != "torch.float32"
-                            or not lse.is_contiguous() or lse.device != kv.device):
+    qs, os_ = _rows_of(q, "attn_paged: q", w, dev), _rows_of(out, "attn_paged: out", w, dev)
+    if lse is not None and not _f32_ok(lse, (T, nh), dev):
         raise ValueError("attn_paged: lse must be a dense [T][nh] fp32")
-    if prefix is not None:
-        _int32(prefix, "attn_paged: prefix", (kv.B,), kv.device)
     if max_keys is None:
         max_keys = kv.cols * kv.page_size
+    wp, wn = None, 0
     if ws is None:
-        n = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys)
-        if n:
+        wn = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys)
+        if wn:
             import torch
-            if stream is not None and stream != torch.cuda.current_stream().cuda_stream:
+            if stream is not None and stream != _raw_stream(dev):
                 raise ValueError("attn_paged: a stream other than torch's current one needs a ws of its own")
-            ws = torch.empty(n, dtype=torch.uint8, device=kv.device)
-    elif ws.device != kv.device or not ws.is_contiguous():
+            ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
+            wp = ws.data_ptr()
+    elif ws.get_device() != dev or not ws.is_contiguous():
         raise ValueError("attn_paged: ws must be a dense tensor on the cache's device")
-    check(lib().gsvk_op_attn_paged(kv._ref, _p(q), T, nh, qs, max_new, max_keys, scale, window, _p(prefix), _p(out),
-                                   _gsvk_type(out.dtype), os_, _p(lse), _p(ws),
-                                   0 if ws is None else ws.numel() * ws.element_size(), _stream(stream)), "attn_paged")
+    else:
+        wp, wn = ws.data_ptr(), ws.numel() * ws.element_size()
+    rc = lib().gsvk_op_attn_paged(kv._ref, q.data_ptr(), T, nh, qs, max_new, max_keys, scale, window,
+                                  None if prefix is None else _int32(prefix, "attn_paged: prefix", (kv.B,), dev),
+                                  out.data_ptr(), _gsvk_type(out.dtype), os_, None if lse is None else lse.data_ptr(),
+                                  wp, wn, st)
+    if rc:
+        check(rc, "attn_paged")
 
 
 def op_sample(logits, cfg, rng, tok_out, hist=None, n_hist=None, probs_out=None, ws=None, stream=None):

@@ -12,6 +12,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#define GSVK_HOSTEMU 1   // (kernels take a builtin where they have loads in asm)
 #define __global__
 #define __device__
 #define __host__

@@ -34,6 +34,7 @@ def check():
     "128 1 17 1 16 0 0 1 0 0 1:130 2:80 20:40",              # groups that are no power of two
     "64 1 10 2 128 0 0 0 0 2 130:400 1:1 1:257 9:9",         # tiles that end inside a page
     "64 0 4 4 16 7 0 0 1 1 33:80 100:300",                   # a window smaller than a tile
+    "64 0 4 2 16 1 0 0 0 0 129:300 40:40",                   # waves whose rows see none of the first tiles
     "32 0 3 3 32 0 200 0 2 0 60:150 1:300",                  # a prefix past the sequence's end
 ], ids=lambda s: s.replace(" ", "_"))
 def test_paged_operators_in_bounds(check, args):
