@@ -468,14 +468,18 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
     __shared__ __align__(16) uint16_t s_v[2][CH_KEYS * HD];
     __shared__ int s_flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
 
-    const int b = blockIdx.z, kvh = blockIdx.y;
-    const int split = blockIdx.x % a.nsplit;
-    const int rt = gridDim.x / a.nsplit - 1 - blockIdx.x / a.nsplit;   // the last rows see the most keys: first
+    // (split, head, sequence) fastest, then the row tiles from each sequence's last, which sees the
+    // most keys, to its first: the longest workgroups start first on every XCD (ids go round-robin
+    // to the 8 XCDs), and with pairs a multiple of 8 an XCD's L2 holds the keys of its own pairs only
+    // (8191 tokens, 8 heads of 128: 777 us with the tiles fastest, the CUs busy for 0.69 of it).
+    const int pairs = a.nsplit * a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
+    const int split = pair % a.nsplit, kvh = pair / a.nsplit % a.kv.n_kv, b = pair / a.nsplit / a.kv.n_kv;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, lh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq s = seq_of(a, b);
+    const int rt = (s.rows + CH_WAVES * 32 - 1) / (CH_WAVES * 32) - 1 - (int) (blockIdx.x / pairs);
     const int r0 = rt * CH_WAVES * 32;
-    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    if (rt < 0 || s.rows < a.min_rows || s.rows > a.max_rows) return;
     const int nh = a.group * a.kv.n_kv;
     // the key ranges of the workgroup and of this wave
     const int tokf = r0 / a.group, tokl = (min(r0 + CH_WAVES * 32, s.rows) - 1) / a.group;
@@ -659,6 +663,14 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
                 asm volatile("" : "+v"(l));   // (summed here: put off, the sum would keep all 32 values live)
                 pf = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
                                          pg_pack<T>(p[6], p[7])));
+                // one product at a time among the vector instructions: in order, a run of products
+                // would hold up the exponentials behind it
+#pragma unroll
+                for (int i = 0; i < NK / 2 + (q > 0 ? DT : 0); i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    if (q > 0) __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2 + DT), 0);
+                    else __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2), 0);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -829,7 +841,7 @@ void launch_attn(PagedAttn a, const Plan & p, hipStream_t st) {
         a.nsplit = p.chunk_split;
         a.min_rows = p.few ? FEW_ROWS + 1 : 1;
         a.max_rows = INT32_MAX;
-        hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) (p.chunk_tiles * p.chunk_split), nkv, B),
+        hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) p.chunk_tiles * p.chunk_split * nkv * B),
                            dim3(CH_WAVES * 64), 0, st, a);
         merge(a.max_new * a.group);
     }
@@ -901,6 +913,8 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     const size_t need = workspace_of(p, tokens * nh, kv->hd);
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
+    GSVK_REQUIRE((int64_t) p.chunk_tiles * p.chunk_split * kv->n_kv * kv->B <= INT32_MAX,
+                 "attn_paged: too many row tiles for one launch");
     a.q = (const uint16_t *) q;
     a.q_stride = q_stride;
     a.out = out;

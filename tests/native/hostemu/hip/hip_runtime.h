@@ -96,6 +96,7 @@ inline void __threadfence() {}
 inline void __threadfence_block() {}
 #define __builtin_amdgcn_fence(...) ((void) 0)
 #define __builtin_amdgcn_sched_barrier(x) ((void) 0)
+#define __builtin_amdgcn_sched_group_barrier(m, n, g) ((void) 0)
 #define __builtin_amdgcn_s_waitcnt(x) ((void) 0)
 #define __builtin_amdgcn_s_barrier() ::emu::barrier()
 inline void __builtin_amdgcn_wave_barrier() { ::emu::wave_sync(); }
