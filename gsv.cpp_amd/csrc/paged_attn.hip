@@ -33,6 +33,7 @@
 // of a tile see a key and others do not, 0 * inf would still give NaN: such blocks are searched
 // for infinities and NaNs, which are taken out of the product and added to the rows that see them
 // (rare; a positive probability times an infinity is that infinity).
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -759,31 +760,58 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
 
 // ---- joining the splits ------------------------------------------------------------------------------
 
-// A workgroup: 16 rows of one (sequence, head); a thread 8 dims of a row at a time
-template <class T, int HD>
+// A workgroup takes 256 / (HD / 8) / SL rows of one (sequence, head); a row's splits are dealt to SL
+// groups of HD / 8 threads, which hold 8 dims each, and the groups are joined through LDS. SL 16
+// where there are more than 4 splits (64 splits of 2 x 64 rows of 128: 54.7 us with SL 1, one split
+// after another).
+template <class T, int HD, int SL>
 __global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
-    constexpr int C = HD / 8;
+    constexpr int C = HD / 8, R = 256 / C / SL;
+    __shared__ float s_x[R][SL][HD + 4];
+    __shared__ float s_ml[R][SL][2];
     const int b = blockIdx.z, kvh = blockIdx.y;
     const Seq s = seq_of(a, b);
-    const int r0 = blockIdx.x * 16;
+    const int r0 = blockIdx.x * R;
     if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
-    const int rr = threadIdx.x / C, col = (threadIdx.x % C) * 8, r = r0 + rr;
-    if (rr >= 16 || r >= s.rows) return;
+    const int rr = threadIdx.x / (C * SL), sl = threadIdx.x / C % SL, col = (threadIdx.x % C) * 8;
+    const int r = min(r0 + rr, s.rows - 1);
     const int nh = a.group * a.kv.n_kv, tok = r / a.group, h = kvh * a.group + r % a.group;
     const int64_t row = s.row0 + tok, id = row * nh + h, step = a.kv.tokens * nh;
     float M = M_NONE, L = 0.0f, x[8] = {};
-    for (int i = 0; i < a.nsplit; i++) M = fmaxf(M, a.part_ml[2 * (i * step + id)]);
-    for (int i = 0; i < a.nsplit; i++) {
+    for (int i = sl; i < a.nsplit; i += SL) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (i * step + id));
-        const float f = __builtin_amdgcn_exp2f(ml.x - M);
         const float4 * p = reinterpret_cast<const float4 *>(a.part_o + (i * step + id) * HD + col);
         const float4 u = p[0], w = p[1];
-        L = __builtin_fmaf(ml.y, f, L);
-        x[0] = __builtin_fmaf(u.x, f, x[0]); x[1] = __builtin_fmaf(u.y, f, x[1]);
-        x[2] = __builtin_fmaf(u.z, f, x[2]); x[3] = __builtin_fmaf(u.w, f, x[3]);
-        x[4] = __builtin_fmaf(w.x, f, x[4]); x[5] = __builtin_fmaf(w.y, f, x[5]);
-        x[6] = __builtin_fmaf(w.z, f, x[6]); x[7] = __builtin_fmaf(w.w, f, x[7]);
+        const float mn = fmaxf(M, ml.x), e = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml.x - mn);
+        M = mn;
+        L = __builtin_fmaf(L, e, ml.y * f);
+        x[0] = __builtin_fmaf(x[0], e, u.x * f); x[1] = __builtin_fmaf(x[1], e, u.y * f);
+        x[2] = __builtin_fmaf(x[2], e, u.z * f); x[3] = __builtin_fmaf(x[3], e, u.w * f);
+        x[4] = __builtin_fmaf(x[4], e, w.x * f); x[5] = __builtin_fmaf(x[5], e, w.y * f);
+        x[6] = __builtin_fmaf(x[6], e, w.z * f); x[7] = __builtin_fmaf(x[7], e, w.w * f);
     }
+    if constexpr (SL > 1) {
+        if (col == 0) {
+            s_ml[rr][sl][0] = M;
+            s_ml[rr][sl][1] = L;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) s_x[rr][sl][col + i] = x[i];
+        __syncthreads();
+        if (sl) return;
+        for (int i = 0; i < SL; i++) M = fmaxf(M, s_ml[rr][i][0]);
+        L = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < SL; k++) {
+            const float f = __builtin_amdgcn_exp2f(s_ml[rr][k][0] - M);
+            L = __builtin_fmaf(s_ml[rr][k][1], f, L);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __builtin_fmaf(s_x[rr][k][col + i], f, x[i]);
+        }
+    }
+    if (r0 + rr >= s.rows) return;
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
@@ -808,8 +836,9 @@ int split_for(int64_t workgroups, int64_t want, int64_t max_keys, int64_t least)
     return n < 1 ? 1 : (int) n;
 }
 
-Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t max_keys) {
+Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
     Plan p{};
+    if (window && max_keys > (int64_t) window + max_new) max_keys = (int64_t) window + max_new;   // (a row tile's)
     if (max_new > tokens) max_new = (int) tokens;
     const int64_t rows = (int64_t) max_new * group;
     p.chunk = rows > FEW_ROWS;
@@ -834,8 +863,12 @@ template <class T, int HD>
 void launch_attn(PagedAttn a, const Plan & p, hipStream_t st) {
     const unsigned nkv = (unsigned) a.kv.n_kv, B = (unsigned) a.kv.B;
     const auto merge = [&](int rows) {
-        if (a.nsplit > 1)
-            hipLaunchKernelGGL((k_attn_paged_merge<T, HD>), dim3((unsigned) ((rows + 15) / 16), nkv, B), dim3(256), 0, st, a);
+        constexpr int R = 256 / (HD / 8);
+        if (a.nsplit > 4)
+            hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 16>), dim3((unsigned) ((rows + R / 16 - 1) / (R / 16)), nkv, B),
+                               dim3(256), 0, st, a);
+        else if (a.nsplit > 1)
+            hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 1>), dim3((unsigned) ((rows + R - 1) / R), nkv, B), dim3(256), 0, st, a);
     };
     if (p.chunk) {
         a.nsplit = p.chunk_split;
@@ -852,7 +885,7 @@ void launch_attn(PagedAttn a, const Plan & p, hipStream_t st) {
         const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
         if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1>), grid, dim3(FEW_WAVES * 64), 0, st, a);
         else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2>), grid, dim3(FEW_WAVES * 64), 0, st, a);
-        merge(FEW_ROWS);
+        merge((int) std::min<int64_t>((int64_t) a.max_new * a.group, FEW_ROWS));
     }
 }
 
@@ -880,11 +913,12 @@ bool attn_args(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new, in
 }  // namespace gsvk
 
 extern "C" size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new,
-                                                  int64_t max_keys) {
+                                                  int64_t max_keys, int window) {
     using namespace gsvk;
-    if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0) return 0;
+    if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0
+        || window < 0) return 0;
     if (kv->hd != 32 && kv->hd != 64 && kv->hd != 128) return 0;
-    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys), tokens * nh, kv->hd);
+    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->hd);
 }
 
 extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
@@ -909,7 +943,7 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
                      && out_stride % (out_type == GSVK_TYPE_F32 ? 4 : 8) == 0,
                  "attn_paged: the rows of q and out must be 16-byte aligned");
     const int group = nh / kv->n_kv;
-    const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys);
+    const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys, window);
     const size_t need = workspace_of(p, tokens * nh, kv->hd);
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);

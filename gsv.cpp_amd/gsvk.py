@@ -171,7 +171,7 @@ def lib():
         L.gsvk_op_sample.argtypes = [vp, i32, i32, vp, i32, vp, C.POINTER(SamplerCfg), vp, vp, vp, vp, vp]
         L.gsvk_op_paged_append.argtypes = [C.POINTER(PagedKVArgs), vp, vp, vp, i32, i64, i32, i64, i64, i64,
                                            C.POINTER(RopeArgs), vp, vp, vp]
-        L.gsvk_attn_paged_workspace_bytes.argtypes = [C.POINTER(PagedKVArgs), i64, i32, i32, i64]
+        L.gsvk_attn_paged_workspace_bytes.argtypes = [C.POINTER(PagedKVArgs), i64, i32, i32, i64, i32]
         L.gsvk_attn_paged_workspace_bytes.restype = C.c_size_t
         L.gsvk_op_attn_paged.argtypes = [C.POINTER(PagedKVArgs), vp, i64, i32, i64, i32, i64, f32, i32, vp, vp, i32,
                                          i64, vp, vp, C.c_size_t, vp]
@@ -477,8 +477,8 @@ def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=Fals
         check(rc, "paged_append")
 
 
-def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys) -> int:
-    return int(lib().gsvk_attn_paged_workspace_bytes(kv._ref, tokens, nh, max_new, max_keys))
+def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys, window=0) -> int:
+    return int(lib().gsvk_attn_paged_workspace_bytes(kv._ref, tokens, nh, max_new, max_keys, window))
 
 
 def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0, prefix=None, ws=None, stream=None):
@@ -498,7 +498,7 @@ def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0,
         max_keys = kv.cols * kv.page_size
     wp, wn = None, 0
     if ws is None:
-        wn = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys)
+        wn = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys, window)
         if wn:
             import torch
             if stream is not None and stream != _raw_stream(dev):

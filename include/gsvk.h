@@ -586,7 +586,7 @@ int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, const void * 
  * nothing in it outlives the call. Results do not depend on what else runs, and are the same bits
  * for the same arguments. */
 size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new,
-                                       int64_t max_keys);
+                                       int64_t max_keys, int window);
 int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
                        int max_new, int64_t max_keys, float scale, int window, const int32_t * prefix,
                        void * out, int out_type, int64_t out_stride, float * lse, void * ws, size_t ws_bytes,

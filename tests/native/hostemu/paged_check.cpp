@@ -147,7 +147,7 @@ int main(int argc, char ** argv) {
                     }
                 }
             }
-    const size_t wsb = gsvk_attn_paged_workspace_bytes(&kv, tokens, nh, max_new, max_keys);
+    const size_t wsb = gsvk_attn_paged_workspace_bytes(&kv, tokens, nh, max_new, max_keys, window);
     void * ws = wsb ? std::malloc(wsb) : nullptr;
     if (ws) std::memset(ws, 0xff, wsb);
     char * out = (char *) std::malloc((size_t) tokens * nh * hd * (f32 ? 4 : 2));

@@ -79,7 +79,7 @@ def test_nothing_to_do_is_no_error():
 
 
 def _ws(kv, tokens, nh, max_new, max_keys):
-    return gsvk.lib().gsvk_attn_paged_workspace_bytes(C.byref(kv), tokens, nh, max_new, max_keys)
+    return gsvk.lib().gsvk_attn_paged_workspace_bytes(C.byref(kv), tokens, nh, max_new, max_keys, 0)
 
 
 def test_workspace_is_asked_for():
@@ -94,4 +94,4 @@ def test_workspace_is_asked_for():
     assert _attn(kv, tokens=1, max_new=1, max_keys=100000, ws=4104, ws_bytes=need) == 1
     assert _ws(kv, 1, 4, 1, 16) == 0
     assert _ws(_kv(hd=48), 1, 4, 1, 100000) == 0      # (arguments that the call itself refuses)
-    assert gsvk.lib().gsvk_attn_paged_workspace_bytes(None, 1, 4, 1, 100000) == 0
+    assert gsvk.lib().gsvk_attn_paged_workspace_bytes(None, 1, 4, 1, 100000, 0) == 0
