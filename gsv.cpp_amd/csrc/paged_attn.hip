@@ -18,8 +18,9 @@
 //                       belongs to the wave, so the loop has no barrier. Bound by HBM.
 //   k_attn_paged_chunk  longer chunks: 8 waves of 32 rows share key tiles of 64 in LDS (double
 //                       buffered), v_mfma_f32_32x32x16.
-// Where a launch would hold too few workgroups, each (sequence, head, row tile) is cut into nsplit
-// runs of keys, whose (maximum, sum, unnormalised output) k_attn_paged_merge joins.
+// Where that makes too few workgroups, or too unequal ones, keys are divided too: k_attn_paged_few cuts
+// each row tile into nsplit runs of keys, k_attn_paged_balanced all row tiles together into equal
+// runs; (maximum, sum, unnormalised output) of the parts are joined by k_attn_paged_merge and _join.
 //
 // Softmax. Exponents are base 2. The reference exponent m of a row is not its running maximum but
 // follows it: it is moved (and O, l rescaled) only when a score exceeds it by more than 2^12, to
@@ -50,9 +51,12 @@ typedef __attribute__((address_space(3))) uint16_t pg_lds1;
 
 constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
 constexpr int FEW_WAVES = 4, FEW_KEYS = 32;
-constexpr int CH_WAVES = 8, CH_KEYS = 64;
+constexpr int CH_WAVES = 8, CH_KEYS = 64, CH_ROWS = CH_WAVES * 32;
 constexpr float M_NONE = -FLT_MAX;    // m of a row that has seen nothing: exp2(score - m) of -inf is 0
 constexpr float M_ROOM = 12.0f, M_SET = 4.0f;
+
+struct BalHead;
+struct BalTile;
 
 struct PagedAttn {
     PagedView kv;
@@ -64,6 +68,8 @@ struct PagedAttn {
     const int32_t * prefix;
     float * part_o;     // [nsplit][tokens * nh][HD]
     float * part_ml;    // [nsplit][tokens * nh][2]
+    BalHead * bal_head;   // k_attn_paged_balanced's (part_o: its slots)
+    BalTile * bal_tiles;
     float scale_log2;
     int group;   // query heads per key/value head
     int window;
@@ -460,30 +466,45 @@ __device__ __forceinline__ void wait_loads() {
     __syncthreads();
 }
 
+// LDS of a workgroup
+template <int HD>
+struct ChunkLds {
+    uint16_t k[2][CH_KEYS * HD];
+    uint16_t v[2][CH_KEYS * HD];
+    int flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
+};
+
+// The key tiles of row tile rt of (s, kvh): the first, and how many (at least one, which may hold
+// nothing that is seen)
+struct Span { int first, num; };
+__device__ __forceinline__ Span span_of(const PagedAttn & a, const Seq & s, int rt) {
+    const int r0 = rt * CH_ROWS;
+    const int klo = key_lo(a, s, r0 / a.group), khi = key_hi(s, (min(r0 + CH_ROWS, s.rows) - 1) / a.group);
+    Span sp;
+    sp.first = klo / CH_KEYS;
+    sp.num = max(1, (khi + CH_KEYS - 1) / CH_KEYS - sp.first);
+    return sp;
+}
+
+// Row tile rt of head kvh of sequence s (index b), key tiles [kt0, kt1) of it. part: null where these
+// are all of them (the output is final), else where the unnormalised output [CH_ROWS][HD] and (maximum,
+// sum) [CH_ROWS][2] go.
 template <class T, int HD>
-__global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn a) {
+__device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, int b, int kvh, int rt, int kt0, int kt1,
+                                           float * part, ChunkLds<HD> & lds) {
     constexpr int C = HD / 8, NT = CH_WAVES * 64;
     constexpr int NK = HD / 16, DT = HD / 32;
     constexpr int NL = C >= CH_WAVES ? C / CH_WAVES : 1;   // direct loads of a wave per tile of K (and of V)
-    __shared__ __align__(16) uint16_t s_k[2][CH_KEYS * HD];
-    __shared__ __align__(16) uint16_t s_v[2][CH_KEYS * HD];
-    __shared__ int s_flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
+    auto & s_k = lds.k;
+    auto & s_v = lds.v;
+    auto & s_flag = lds.flag;
 
-    // (split, head, sequence) fastest, then the row tiles from each sequence's last, which sees the
-    // most keys, to its first: the longest workgroups start first on every XCD (ids go round-robin
-    // to the 8 XCDs), and with pairs a multiple of 8 an XCD's L2 holds the keys of its own pairs only
-    // (8191 tokens, 8 heads of 128: 777 us with the tiles fastest, the CUs busy for 0.69 of it).
-    const int pairs = a.nsplit * a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
-    const int split = pair % a.nsplit, kvh = pair / a.nsplit % a.kv.n_kv, b = pair / a.nsplit / a.kv.n_kv;
+    const int r0 = rt * CH_ROWS;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, lh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Seq s = seq_of(a, b);
-    const int rt = (s.rows + CH_WAVES * 32 - 1) / (CH_WAVES * 32) - 1 - (int) (blockIdx.x / pairs);
-    const int r0 = rt * CH_WAVES * 32;
-    if (rt < 0 || s.rows < a.min_rows || s.rows > a.max_rows) return;
     const int nh = a.group * a.kv.n_kv;
     // the key ranges of the workgroup and of this wave
-    const int tokf = r0 / a.group, tokl = (min(r0 + CH_WAVES * 32, s.rows) - 1) / a.group;
+    const int tokf = r0 / a.group, tokl = (min(r0 + CH_ROWS, s.rows) - 1) / a.group;
     const int klo = key_lo(a, s, tokf), khi = key_hi(s, tokl);
     const int lo_max = key_lo(a, s, tokl), hi_min = key_hi(s, tokf);
     const int rw = r0 + wave * 32;
@@ -500,9 +521,6 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
 #pragma unroll
         for (int c = 0; c < NK; c++) qf[c] = v8_of<T>(*reinterpret_cast<const uint4 *>(qp + 16 * c));
     }
-    const int kt_a = klo / CH_KEYS, nkt = khi > klo ? (khi + CH_KEYS - 1) / CH_KEYS - kt_a : 0;
-    const int per = (nkt + a.nsplit - 1) / a.nsplit;
-    const int kt0 = kt_a + min(nkt, split * per), kt1 = kt_a + min(nkt, (split + 1) * per);
     const int32_t * tb = a.kv.table + b * a.kv.table_stride;
 
     // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (8 j + wave) * 64 on
@@ -734,7 +752,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
     l = sum_x32(l);
     if (rw + li >= s.rows) return;
     const int64_t row = s.row0 + tok, id = row * nh + h;
-    if (a.nsplit == 1) {
+    if (!part) {
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; d++)
@@ -747,15 +765,186 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn
             }
         if (a.lse && lh == 0) a.lse[id] = lse_of(m, l);
     } else {
-        const int64_t at = (int64_t) split * a.kv.tokens * nh + id;
+        const int rl = wave * 32 + li;
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int v = 0; v < 16; v += 4)
-                *reinterpret_cast<float4 *>(a.part_o + at * HD + 32 * d + 2 * v + 4 * lh) =
+                *reinterpret_cast<float4 *>(part + rl * HD + 32 * d + 2 * v + 4 * lh) =
                     make_float4(o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]);
-        if (lh == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * at) = make_float2(m, l);
+        if (lh == 0) *reinterpret_cast<float2 *>(part + CH_ROWS * HD + 2 * rl) = make_float2(m, l);
     }
+}
+
+// One row tile per workgroup, all its keys. (head, sequence) fastest, then the row tiles from each
+// sequence's last, which sees the most keys, to its first: the longest workgroups start first on
+// every XCD (ids go round-robin to the 8 XCDs), and with pairs a multiple of 8 an XCD's L2 holds the
+// keys of its own pairs only (8191 tokens, 8 heads of 128: 777 us with the tiles fastest, the CUs busy
+// for 0.69 of it; 594 us so).
+template <class T, int HD>
+__global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn a) {
+    __shared__ __align__(16) ChunkLds<HD> lds;
+    const int pairs = a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
+    const int kvh = pair % a.kv.n_kv, b = pair / a.kv.n_kv;
+    const Seq s = seq_of(a, b);
+    const int rt = (s.rows + CH_ROWS - 1) / CH_ROWS - 1 - (int) (blockIdx.x / pairs);
+    if (rt < 0 || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    const Span sp = span_of(a, s, rt);
+    chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds);
+}
+
+// Few row tiles of unequal length: the key tiles of all of them, in the order (head, sequence, row
+// tile, key), are cut into equal runs, one per workgroup (CUs that would wait for the longest row
+// tile share its keys). A row tile that a cut goes through is joined by k_attn_paged_join. Every workgroup computes
+// the same list of row tiles and running sums; the ids of an XCD take consecutive runs.
+constexpr int BAL_GROUPS = 256, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
+
+struct BalHead { int tiles, run; };                 // row tiles of a head, key tiles per workgroup
+struct BalTile { int first, num, b, rt; };          // a row tile's place in its head's list of key tiles
+template <int HD>
+constexpr size_t bal_slot() { return (size_t) CH_ROWS * (HD + 2); }   // floats
+
+struct BalLds {
+    int tiles[BAL_SEQS + 1];    // row tiles before each sequence
+    int units[BAL_TILES + 1];   // key tiles before each row tile of a head
+    int wave[CH_WAVES];
+};
+
+// Exclusive prefix sums of x over the workgroup's threads; total to every thread. Two barriers.
+__device__ __forceinline__ int scan512(int x, int * s_wave, int & total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int y = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int z = __shfl_up(y, d, 64);
+        if (lane >= d) y += z;
+    }
+    if (lane == 63) s_wave[wave] = y;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < CH_WAVES; w++) {
+        if (w < wave) before += s_wave[w];
+        total += s_wave[w];
+    }
+    __syncthreads();
+    return before + y - x;
+}
+// the last i in [0, n) with p[i] <= x (p ascending, p[0] <= x)
+__device__ __forceinline__ int last_le(const int * p, int n, int x) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <class T, int HD>
+__global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedAttn a) {
+    __shared__ __align__(16) ChunkLds<HD> lds;
+    __shared__ BalLds bal;
+    const int tid = threadIdx.x;
+    // row tiles of the sequences
+    int tiles = 0;
+    {
+        int n = 0;
+        if (tid < a.kv.B) {
+            const Seq s = seq_of(a, tid);
+            if (s.rows >= a.min_rows && s.rows <= a.max_rows) n = (s.rows + CH_ROWS - 1) / CH_ROWS;
+        }
+        n = scan512(n, bal.wave, tiles);
+        if (tid < a.kv.B) bal.tiles[tid] = n;
+        if (tid == 0) bal.tiles[a.kv.B] = tiles;
+        tiles = min(tiles, BAL_TILES);   // (the plan has made sure)
+        __syncthreads();
+    }
+    if (tiles == 0) {
+        if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{0, 1};
+        return;
+    }
+    tiles = __builtin_amdgcn_readfirstlane(tiles);
+    int units = 0;   // key tiles of a head
+    for (int e0 = 0; e0 < tiles; e0 += CH_WAVES * 64) {
+        int n = 0, add = 0;
+        const int e = e0 + tid;
+        if (e < tiles) {
+            const int b = last_le(bal.tiles, a.kv.B, e);
+            n = span_of(a, seq_of(a, b), e - bal.tiles[b]).num;
+        }
+        n = scan512(n, bal.wave, add);
+        if (e < tiles) bal.units[e] = units + n;
+        units += add;
+    }
+    if (tid == 0) bal.units[tiles] = units;
+    __syncthreads();
+    units = __builtin_amdgcn_readfirstlane(units);
+    const int64_t total = (int64_t) units * a.kv.n_kv;
+    const int64_t share = (total + BAL_GROUPS - 1) / BAL_GROUPS;
+    const int run = (int) max(share, (int64_t) min(BAL_LEAST, (units + tiles - 1) / tiles));
+    if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{tiles, run};
+
+    const int w = (int) (blockIdx.x % 8) * (BAL_GROUPS / 8) + (int) (blockIdx.x / 8);
+    const int64_t u0 = (int64_t) w * run, u1 = min(total, u0 + run);
+    for (int64_t u = u0; u < u1;) {
+        // (all uniform; said so for the direct loads, whose base is scalar)
+        const int kvh = __builtin_amdgcn_readfirstlane((int) (u / units)), at = __builtin_amdgcn_readfirstlane((int) (u % units));
+        const int e = __builtin_amdgcn_readfirstlane(last_le(bal.units, tiles, at));
+        const int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
+        const int rt = __builtin_amdgcn_readfirstlane(e - bal.tiles[b]);
+        const int first = __builtin_amdgcn_readfirstlane(bal.units[e]);
+        const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first, t0 = at - first;
+        const int t1 = __builtin_amdgcn_readfirstlane((int) min((int64_t) num, t0 + (u1 - u)));
+        const Seq s = seq_of(a, b);
+        const Span sp = span_of(a, s, rt);
+        float * part = nullptr;
+        if (t1 - t0 < num) part = a.part_o + (int64_t) (2 * w + (u > u0)) * bal_slot<HD>();
+        if (t0 == 0 && tid == 0) a.bal_tiles[kvh * tiles + e] = BalTile{first, num, b, rt};
+        chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first + t0, sp.first + t1, part, lds);
+        u += t1 - t0;
+        __syncthreads();   // (the next row tile's loads overwrite this one's LDS)
+    }
+}
+
+// The row tiles that k_attn_paged_balanced has cut: workgroup = (256 / (HD / 8) rows, row tile, head), a
+// thread 8 dims of a row
+template <class T, int HD>
+__global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
+    constexpr int C = HD / 8, R = 256 / C;
+    const BalHead hd = *a.bal_head;
+    const int e = blockIdx.y, kvh = blockIdx.z;
+    if (e >= hd.tiles) return;
+    const BalTile t = a.bal_tiles[kvh * hd.tiles + e];
+    // (a head's key tiles follow the last head's)
+    const BalTile last = a.bal_tiles[hd.tiles - 1];
+    const int64_t u0 = (int64_t) kvh * (last.first + last.num) + t.first, u1 = u0 + t.num;
+    const int64_t w0 = u0 / hd.run, w1 = (u1 - 1) / hd.run;
+    if (w0 == w1) return;
+    const Seq s = seq_of(a, t.b);
+    const int rl = blockIdx.x * R + threadIdx.x / C, col = (threadIdx.x % C) * 8, r = t.rt * CH_ROWS + rl;
+    if (r >= s.rows) return;
+    float M = M_NONE, L = 0.0f, x[8] = {};
+    for (int64_t w = w0; w <= w1; w++) {
+        const float * part = a.part_o + (2 * w + (w * hd.run < u0)) * bal_slot<HD>();
+        const float2 ml = *reinterpret_cast<const float2 *>(part + CH_ROWS * HD + 2 * rl);
+        const float4 * p = reinterpret_cast<const float4 *>(part + rl * HD + col);
+        const float4 u = p[0], v = p[1];
+        const float mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml.x - mn);
+        M = mn;
+        L = __builtin_fmaf(L, c, ml.y * f);
+        x[0] = __builtin_fmaf(x[0], c, u.x * f); x[1] = __builtin_fmaf(x[1], c, u.y * f);
+        x[2] = __builtin_fmaf(x[2], c, u.z * f); x[3] = __builtin_fmaf(x[3], c, u.w * f);
+        x[4] = __builtin_fmaf(x[4], c, v.x * f); x[5] = __builtin_fmaf(x[5], c, v.y * f);
+        x[6] = __builtin_fmaf(x[6], c, v.z * f); x[7] = __builtin_fmaf(x[7], c, v.w * f);
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
+    const int tok = r / a.group, h = kvh * a.group + r % a.group;
+    store8<T>(a, s.row0 + tok, h * HD + col, x);
+    if (a.lse && col == 0) a.lse[(s.row0 + tok) * a.group * a.kv.n_kv + h] = lse_of(M, L);
 }
 
 // ---- joining the splits ------------------------------------------------------------------------------
@@ -825,21 +1014,14 @@ __global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
 struct Plan {
     bool few, chunk;
     int few_qt, few_tiles, few_split;
-    int chunk_tiles, chunk_split;
+    int chunk_tiles;       // row tiles of the longest sequence
+    int balanced_tiles;    // 0: one row tile per workgroup; else the most row tiles that there can be per head
 };
-
-int split_for(int64_t workgroups, int64_t want, int64_t max_keys, int64_t least) {
-    int64_t n = (want + workgroups - 1) / workgroups;
-    const int64_t most = max_keys / least;
-    if (n > most) n = most;
-    if (n > 64) n = 64;
-    return n < 1 ? 1 : (int) n;
-}
 
 Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
     Plan p{};
-    if (window && max_keys > (int64_t) window + max_new) max_keys = (int64_t) window + max_new;   // (a row tile's)
     if (max_new > tokens) max_new = (int) tokens;
+    if (window && max_keys > (int64_t) window + max_new) max_keys = (int64_t) window + max_new;   // (a row tile's)
     const int64_t rows = (int64_t) max_new * group;
     p.chunk = rows > FEW_ROWS;
     p.few = !p.chunk || (B > 1 && group <= FEW_ROWS);
@@ -847,61 +1029,73 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
         const int64_t most = rows < FEW_ROWS ? rows : FEW_ROWS;
         p.few_qt = most <= 16 || (p.chunk && group <= 16) ? 1 : 2;
         p.few_tiles = (int) ((most + 16 * p.few_qt - 1) / (16 * p.few_qt));
-        p.few_split = split_for((int64_t) B * n_kv, 1024, max_keys, 256);
+        const int64_t n = std::min((1024 + (int64_t) B * n_kv - 1) / ((int64_t) B * n_kv), max_keys / 256);
+        p.few_split = (int) std::max<int64_t>(1, std::min<int64_t>(n, 64));
     }
     if (p.chunk) {
-        constexpr int R = CH_WAVES * 32;
-        p.chunk_tiles = (int) ((rows + R - 1) / R);
-        int64_t tiles = tokens * group / R;   // of all sequences, about
-        if (tiles < 1) tiles = 1;
-        p.chunk_split = split_for(tiles * n_kv, 256, max_keys, 512);
+        p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);
+        // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence
+        const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS), most = tokens * group / CH_ROWS + B;
+        const bool enough = least * n_kv >= 768 || (least * n_kv >= 192 && max_keys <= 1024) || max_keys <= 256;
+        if (!enough && B <= BAL_SEQS && most <= BAL_TILES) p.balanced_tiles = (int) most;
     }
     return p;
 }
 
+size_t bal_tables(const Plan & p, int n_kv) {   // bytes before the slots
+    const size_t n = sizeof(BalHead) + (size_t) p.balanced_tiles * n_kv * sizeof(BalTile);
+    return (n + 255) / 256 * 256;
+}
+
 template <class T, int HD>
-void launch_attn(PagedAttn a, const Plan & p, hipStream_t st) {
+void launch_attn(PagedAttn a, const Plan & p, void * ws, hipStream_t st) {
     const unsigned nkv = (unsigned) a.kv.n_kv, B = (unsigned) a.kv.B;
-    const auto merge = [&](int rows) {
+    if (p.chunk) {
+        a.min_rows = p.few ? FEW_ROWS + 1 : 1;
+        a.max_rows = INT32_MAX;
+        if (p.balanced_tiles) {
+            a.bal_head = (BalHead *) ws;
+            a.bal_tiles = (BalTile *) (a.bal_head + 1);
+            a.part_o = (float *) ((char *) ws + bal_tables(p, a.kv.n_kv));
+            hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), dim3(BAL_GROUPS), dim3(CH_WAVES * 64), 0, st, a);
+            hipLaunchKernelGGL((k_attn_paged_join<T, HD>), dim3(CH_ROWS / (256 / (HD / 8)), (unsigned) p.balanced_tiles, nkv),
+                               dim3(256), 0, st, a);
+        } else {
+            hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) p.chunk_tiles * nkv * B), dim3(CH_WAVES * 64), 0, st, a);
+        }
+    }
+    if (p.few) {   // (after the chunks: their part of the workspace is free again)
+        a.nsplit = p.few_split;
+        a.min_rows = 1;
+        a.max_rows = FEW_ROWS;
+        a.part_o = (float *) ws;
+        a.part_ml = a.part_o + (size_t) p.few_split * a.kv.tokens * a.group * nkv * HD;
+        const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
+        if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1>), grid, dim3(FEW_WAVES * 64), 0, st, a);
+        else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2>), grid, dim3(FEW_WAVES * 64), 0, st, a);
         constexpr int R = 256 / (HD / 8);
+        const int rows = (int) std::min<int64_t>((int64_t) a.max_new * a.group, FEW_ROWS);
         if (a.nsplit > 4)
             hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 16>), dim3((unsigned) ((rows + R / 16 - 1) / (R / 16)), nkv, B),
                                dim3(256), 0, st, a);
         else if (a.nsplit > 1)
             hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 1>), dim3((unsigned) ((rows + R - 1) / R), nkv, B), dim3(256), 0, st, a);
-    };
-    if (p.chunk) {
-        a.nsplit = p.chunk_split;
-        a.min_rows = p.few ? FEW_ROWS + 1 : 1;
-        a.max_rows = INT32_MAX;
-        hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) p.chunk_tiles * p.chunk_split * nkv * B),
-                           dim3(CH_WAVES * 64), 0, st, a);
-        merge(a.max_new * a.group);
-    }
-    if (p.few) {
-        a.nsplit = p.few_split;
-        a.min_rows = 1;
-        a.max_rows = FEW_ROWS;
-        const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
-        if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1>), grid, dim3(FEW_WAVES * 64), 0, st, a);
-        else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2>), grid, dim3(FEW_WAVES * 64), 0, st, a);
-        merge((int) std::min<int64_t>((int64_t) a.max_new * a.group, FEW_ROWS));
     }
 }
 
 template <class T>
-void launch_attn(const PagedAttn & a, int hd, const Plan & p, hipStream_t st) {
-    if (hd == 32) launch_attn<T, 32>(a, p, st);
-    else if (hd == 64) launch_attn<T, 64>(a, p, st);
-    else launch_attn<T, 128>(a, p, st);
+void launch_attn(const PagedAttn & a, int hd, const Plan & p, void * ws, hipStream_t st) {
+    if (hd == 32) launch_attn<T, 32>(a, p, ws, st);
+    else if (hd == 64) launch_attn<T, 64>(a, p, ws, st);
+    else launch_attn<T, 128>(a, p, ws, st);
 }
 
-// bytes of a split's partial results: rows x (HD outputs, maximum, sum)
-size_t workspace_of(const Plan & p, int64_t rows, int hd) {
-    int n = 1;
-    if (p.few && p.few_split > n) n = p.few_split;
-    if (p.chunk && p.chunk_split > n) n = p.chunk_split;
-    return n > 1 ? (size_t) n * (size_t) rows * (size_t) (hd + 2) * sizeof(float) : 0;
+// bytes of partial results: the splits' rows x (hd outputs, maximum, sum), the cut row tiles' slots
+size_t workspace_of(const Plan & p, int64_t rows, int n_kv, int hd) {
+    size_t few = 0, bal = 0;
+    if (p.few && p.few_split > 1) few = (size_t) p.few_split * (size_t) rows * (size_t) (hd + 2) * sizeof(float);
+    if (p.balanced_tiles) bal = bal_tables(p, n_kv) + 2 * (size_t) BAL_GROUPS * CH_ROWS * (size_t) (hd + 2) * sizeof(float);
+    return few > bal ? few : bal;
 }
 
 bool attn_args(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new, int64_t max_keys) {
@@ -918,7 +1112,7 @@ extern "C" size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int6
     if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0
         || window < 0) return 0;
     if (kv->hd != 32 && kv->hd != 64 && kv->hd != 128) return 0;
-    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->hd);
+    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->n_kv, kv->hd);
 }
 
 extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
@@ -944,10 +1138,10 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
                  "attn_paged: the rows of q and out must be 16-byte aligned");
     const int group = nh / kv->n_kv;
     const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys, window);
-    const size_t need = workspace_of(p, tokens * nh, kv->hd);
+    const size_t need = workspace_of(p, tokens * nh, kv->n_kv, kv->hd);
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
-    GSVK_REQUIRE((int64_t) p.chunk_tiles * p.chunk_split * kv->n_kv * kv->B <= INT32_MAX,
+    GSVK_REQUIRE((int64_t) p.chunk_tiles * kv->n_kv * kv->B <= INT32_MAX,
                  "attn_paged: too many row tiles for one launch");
     a.q = (const uint16_t *) q;
     a.q_stride = q_stride;
@@ -960,13 +1154,8 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     a.window = window;
     a.max_new = max_new < tokens ? max_new : (int) tokens;
     a.out_f32 = out_type == GSVK_TYPE_F32;
-    if (need) {
-        const int n = (int) (need / ((size_t) tokens * nh * (kv->hd + 2) * sizeof(float)));
-        a.part_o = (float *) ws;
-        a.part_ml = a.part_o + (size_t) n * tokens * nh * kv->hd;
-    }
-    if (kv->type == GSVK_TYPE_F16) launch_attn<PgF16>(a, kv->hd, p, (hipStream_t) stream);
-    else launch_attn<PgBF16>(a, kv->hd, p, (hipStream_t) stream);
+    if (kv->type == GSVK_TYPE_F16) launch_attn<PgF16>(a, kv->hd, p, ws, (hipStream_t) stream);
+    else launch_attn<PgBF16>(a, kv->hd, p, ws, (hipStream_t) stream);
     GSVK_LAUNCH_CHECK();
     return GSVK_OK;
 }

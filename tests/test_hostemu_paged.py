@@ -27,6 +27,8 @@ def check():
     "32 0 4 4 16 0 0 0 0 2 1:1 1:40 1:300 3:70 0:9 0:0",     # single tokens and a draft
     "64 1 8 2 32 0 0 1 0 0 1:3000",                          # split over the keys and joined
     "128 1 2 1 16 0 0 0 0 1 90:1400",                        # a chunk split over the keys
+    "32 0 4 2 16 0 0 0 1 2 300:1500 1:40 0:0 40:900 200:200 129:700",   # unequal row tiles cut into equal runs
+    "64 1 8 1 32 0 0 0 0 0 33:3000 70:90",
     "128 0 4 1 16 0 0 0 0 1 1:100 90:200 0:7 1:33",          # a mix
     "128 1 6 2 16 50 0 0 1 0 40:97 70:70",                   # a window; NaN in each chunk's last key
     "32 0 2 2 64 0 60 0 2 3 100:130 1:500",                  # a prefix; entries that name no page
