@@ -12,7 +12,7 @@
 // by the transposing 16-bit read, four keys of one dim per lane).
 //
 //   k_attn_paged_few    sequences of at most 32 rows (single tokens, drafts): the keys are dealt to
-//                       the 4 waves of a workgroup in blocks of 32, each wave with its own running
+//                       the 4 or 8 waves of a workgroup in blocks of 32, each wave with its own running
 //                       maximum and sum; K goes straight into the operand registers
 //                       (v_mfma_f32_16x16x32: 16 keys x 32 dims), V through a tile of LDS that
 //                       belongs to the wave, so the loop has no barrier. Bound by HBM.
@@ -48,9 +48,10 @@ typedef float pg_f16 __attribute__((ext_vector_type(16)));
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pg_s4 pg_lds4;
 typedef __attribute__((address_space(3))) uint16_t pg_lds1;
+typedef const __attribute__((address_space(4))) int32_t pg_table;   // (no store of these kernels reaches it: scalar loads)
 
 constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
-constexpr int FEW_WAVES = 4, FEW_KEYS = 32;
+constexpr int FEW_KEYS = 32;
 constexpr int CH_WAVES = 8, CH_KEYS = 64, CH_ROWS = CH_WAVES * 32;
 constexpr float M_NONE = -FLT_MAX;    // m of a row that has seen nothing: exp2(score - m) of -inf is 0
 constexpr float M_ROOM = 12.0f, M_SET = 4.0f;
@@ -177,7 +178,7 @@ __device__ __forceinline__ int key_hi(const Seq & s, int tok) {
 }
 
 // Page of a key (uniform over the wave), -1 if it has none
-__device__ __forceinline__ int page_of(const PagedAttn & a, const int32_t * tb, int key) {
+__device__ __forceinline__ int page_of(const PagedAttn & a, pg_table * tb, int key) {
     const int col = key >> a.kv.page_shift;
     const int pg = col < a.kv.table_cols ? tb[col] : -1;
     return pg >= 0 && pg < a.kv.n_pages ? pg : -1;
@@ -215,13 +216,13 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 
 // ---- few rows ------------------------------------------------------------------------------------
 
-// QT tiles of 16 rows per workgroup
-template <class T, int HD, int QT>
-__global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) {
+// QT tiles of 16 rows per workgroup of NW waves
+template <class T, int HD, int QT, int NW>
+__global__ void __launch_bounds__(NW * 64) k_attn_paged_few(PagedAttn a) {
     constexpr int C = HD / 8, NV = FEW_KEYS * C / 64, NK = HD / 32, DT = HD / 16, OS = HD + 4;
     constexpr int VB = FEW_KEYS * HD * 2, OB = 16 * OS * 4;   // LDS bytes of a wave: V tile, outputs
-    __shared__ __align__(16) char s_mem[FEW_WAVES * (VB > OB ? VB : OB)];
-    __shared__ float s_ml[FEW_WAVES][QT * 16][2];
+    __shared__ __align__(16) char s_mem[NW * (VB > OB ? VB : OB)];
+    __shared__ float s_ml[NW][QT * 16][2];
 
     const int b = blockIdx.z, kvh = blockIdx.y;
     const int split = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
     const int per = (nblk + a.nsplit - 1) / a.nsplit;
     const int blk0 = blk_a + min(nblk, split * per), blk1 = blk_a + min(nblk, (split + 1) * per);
 
-    const int32_t * tb = a.kv.table + b * a.kv.table_stride;
+    pg_table * tb = (pg_table *) (a.kv.table + b * a.kv.table_stride);
     uint16_t * sv = reinterpret_cast<uint16_t *>(s_mem + wave * VB);
     uint4 kr[2][NK], vr[NV];
     int pg[2];
@@ -284,12 +285,12 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
         pg[1] = page_of(a, tb, blk * FEW_KEYS + 16);
         fetch(blk, pg);
     }
-    for (; blk < blk1; blk += FEW_WAVES) {
+    for (; blk < blk1; blk += NW) {
         const int kb = blk * FEW_KEYS;
         const bool ok0 = pg[0] >= 0, ok1 = pg[1] >= 0;
         const bool full = kb >= lo_max && kb + FEW_KEYS <= hi_min && ok0 && ok1;
         // the next block's pages
-        const int nb = blk + FEW_WAVES < blk1 ? blk + FEW_WAVES : blk;
+        const int nb = blk + NW < blk1 ? blk + NW : blk;
         const int np[2] = {page_of(a, tb, nb * FEW_KEYS), page_of(a, tb, nb * FEW_KEYS + 16)};
         bool odd = false;
         if (!full) {
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
         if (t) __syncthreads();
         float M = s_ml[0][t * 16 + li][0];
 #pragma unroll
-        for (int w = 1; w < FEW_WAVES; w++) M = fmaxf(M, s_ml[w][t * 16 + li][0]);
+        for (int w = 1; w < NW; w++) M = fmaxf(M, s_ml[w][t * 16 + li][0]);
         const float f = __builtin_amdgcn_exp2f(s_ml[wave][t * 16 + li][0] - M);
 #pragma unroll
         for (int d = 0; d < DT; d++) {
@@ -419,9 +420,9 @@ __global__ void __launch_bounds__(FEW_WAVES * 64) k_attn_paged_few(PagedAttn a) 
             const int tok = r / a.group, h = kvh * a.group + r % a.group;
             float Mr = M_NONE, L = 0.0f, x[8] = {};
 #pragma unroll
-            for (int w = 0; w < FEW_WAVES; w++) Mr = fmaxf(Mr, s_ml[w][t * 16 + rr][0]);
+            for (int w = 0; w < NW; w++) Mr = fmaxf(Mr, s_ml[w][t * 16 + rr][0]);
 #pragma unroll
-            for (int w = 0; w < FEW_WAVES; w++) {
+            for (int w = 0; w < NW; w++) {
                 L += s_ml[w][t * 16 + rr][1] * __builtin_amdgcn_exp2f(s_ml[w][t * 16 + rr][0] - Mr);
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] += so[(w * 16 + rr) * OS + col + i];
@@ -460,17 +461,26 @@ __device__ __forceinline__ void load_lds(const char * base, uint32_t off, uint16
                  : "memory");
 #endif
 }
-// every load of this wave has landed, every LDS operation of it is done; then all waves' are
+// All but the last N loads of this wave have landed, every LDS operation of it is done (gfx9
+// encoding: vmcnt in bits 3:0 and 15:14, lgkmcnt in 11:8, expcnt not waited on); then all waves' are.
+// In order: other loads of the wave, before or after these, only make it wait longer.
+template <int N>
 __device__ __forceinline__ void wait_loads() {
-    __builtin_amdgcn_s_waitcnt(0x7 << 4);   // gfx9: vmcnt 0, lgkmcnt 0, expcnt not waited on
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
+#ifdef GSVK_HOSTEMU
     __syncthreads();
+#else
+    asm volatile("s_barrier" ::: "memory");
+#endif
 }
 
 // LDS of a workgroup
 template <int HD>
+constexpr int ch_ahead() { return HD == 128 ? 1 : 3; }   // tiles of V in flight beyond the current one (K: one more)
+template <int HD>
 struct ChunkLds {
-    uint16_t k[2][CH_KEYS * HD];
-    uint16_t v[2][CH_KEYS * HD];
+    uint16_t k[ch_ahead<HD>() + 1][CH_KEYS * HD];
+    uint16_t v[ch_ahead<HD>() + 1][CH_KEYS * HD];
     int flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
 };
 
@@ -495,6 +505,8 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
     constexpr int C = HD / 8, NT = CH_WAVES * 64;
     constexpr int NK = HD / 16, DT = HD / 32;
     constexpr int NL = C >= CH_WAVES ? C / CH_WAVES : 1;   // direct loads of a wave per tile of K (and of V)
+    constexpr int AHEAD = ch_ahead<HD>(), NB = AHEAD + 1;
+    constexpr int FLY = (HD > 32 ? 2 : 1) * NL * (AHEAD - 1);   // a wave's loads that a step leaves in flight
     auto & s_k = lds.k;
     auto & s_v = lds.v;
     auto & s_flag = lds.flag;
@@ -521,7 +533,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
 #pragma unroll
         for (int c = 0; c < NK; c++) qf[c] = v8_of<T>(*reinterpret_cast<const uint4 *>(qp + 16 * c));
     }
-    const int32_t * tb = a.kv.table + b * a.kv.table_stride;
+    pg_table * tb = (pg_table *) (a.kv.table + b * a.kv.table_stride);
 
     // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (8 j + wave) * 64 on
     // (all within one group of 16 keys, one page); with 32 dims waves 0-3 load K, 4-7 V.
@@ -532,14 +544,20 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
         off_k[j] = ((key & 15) * HD + (((u % C) ^ swz_k<HD>(key)) << 3)) * 2;
         off_v[j] = ((key & 15) * HD + (((u % C) ^ swz_vc<HD>(key)) << 3)) * 2;
     }
-    int64_t at_v[NL] = {};   // byte offsets of the wave's key groups in the tile whose V comes next
-    const auto offsets = [&](int kt, int64_t (&at)[NL]) {
-#pragma unroll
-        for (int j = 0; j < NL; j++) {
-            const int key = kt * CH_KEYS + ((j * CH_WAVES + wave) % C) * (CH_KEYS / C) / 16 * 16;
-            at[j] = key_at<HD>(a, page_of(a, tb, key), kvh, key) * 2;
-        }
+    // pages of the wave's key groups in tile kt (past the last tile: that tile's), and their byte offsets
+    const auto group_of = [&](int kt, int j) {
+        return min(kt, kt1 - 1) * CH_KEYS + ((j * CH_WAVES + wave) % C) * (CH_KEYS / C) / 16 * 16;
     };
+    const auto pages = [&](int kt, int (&pg)[NL]) {
+#pragma unroll
+        for (int j = 0; j < NL; j++) pg[j] = page_of(a, tb, group_of(kt, j));
+    };
+    const auto offsets = [&](int kt, const int (&pg)[NL], int64_t (&at)[NL]) {
+#pragma unroll
+        for (int j = 0; j < NL; j++) at[j] = key_at<HD>(a, pg[j], kvh, group_of(kt, j)) * 2;
+    };
+    int pg_n[NL] = {};       // pages of the tile whose K comes next: read a step ahead
+    int64_t at_v[NL] = {};   // offsets of the tile whose V comes next
     const auto load = [&](const uint16_t * cache, const int64_t (&at)[NL], const uint32_t (&off)[NL], uint16_t * lds) {
 #pragma unroll
         for (int j = 0; j < NL; j++)
@@ -643,10 +661,13 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             }
             __syncthreads();
         }
-        if (kt + 1 < kt1) load_v(at_v, buf ^ 1);
-        if (kt + 2 < kt1) {
-            offsets(kt + 2, at_v);
+        // V of tile kt + AHEAD, K of the one after it, into the buffers that step kt - 1 read. Past the last tile
+        // nothing (AHEAD 1), or the last one again: the count of loads in flight stays the same.
+        if (AHEAD > 1 || kt + AHEAD < kt1) load_v(at_v, (buf + AHEAD) % NB);
+        if (AHEAD > 1 || kt + AHEAD + 1 < kt1) {
+            offsets(kt + AHEAD + 1, pg_n, at_v);
             load_k(at_v, buf);
+            pages(kt + AHEAD + 2, pg_n);
         }
         if (kb < whi && kb + 2 * CH_KEYS > wlo) {   // a row of the wave sees this tile, or the next one
             top *= a.scale_log2;
@@ -662,10 +683,10 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             }
             uint4 kf[2][NK / 2];
             typename T::v8 vf[2][DT], pf;
-            read_k(kf[0], buf ^ 1, 0);
+            read_k(kf[0], (buf + 1) % NB, 0);
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                if (q < 3) read_k(kf[(q + 1) & 1], buf ^ 1, q + 1);
+                if (q < 3) read_k(kf[(q + 1) & 1], (buf + 1) % NB, q + 1);
                 read_v(vf[q & 1], buf, q);
                 mul_k(sn, kf[q & 1], q);
                 if (q > 0) {
@@ -713,7 +734,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             if (!(kb + CH_KEYS >= wlo_max && kb + 2 * CH_KEYS <= whi_min && !has_bad)) mask(sn, kt + 1);
             top = top_of(sn);
         }
-        wait_loads();
+        wait_loads<FLY>();   // V of the next tile and K of the one after it are there
     };
 
     if (kt0 < kt1) {
@@ -723,13 +744,19 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
         const int c0 = (kt0 * CH_KEYS) >> a.kv.page_shift, c1 = (min(kt1 * CH_KEYS, khi) - 1) >> a.kv.page_shift;
         for (int c = c0 + tid; c <= c1; c += NT)
             if (page_of(a, tb, c << a.kv.page_shift) < 0) s_flag[0] = 1;
-        int64_t at[NL];
-        offsets(kt0, at);
-        load_k(at, 0);
-        load_v(at, 0);
-        offsets(min(kt0 + 1, kt1 - 1), at_v);
-        load_k(at_v, 1);
-        wait_loads();
+        int pg[NB][NL];
+#pragma unroll
+        for (int i = 0; i < NB; i++) pages(kt0 + i, pg[i]);
+        pages(kt0 + NB, pg_n);
+        offsets(kt0, pg[0], at_v);
+        load_k(at_v, 0);
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+            load_v(at_v, i);
+            offsets(kt0 + i + 1, pg[i + 1], at_v);
+            load_k(at_v, i + 1);
+        }
+        wait_loads<FLY>();
         has_bad = __builtin_amdgcn_readfirstlane(s_flag[0]) != 0;
         // (a wave whose rows see none of the first tiles passes over them: its scores are then these)
         pg_f16 s0[2], s1[2];
@@ -742,10 +769,15 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             top = top_of(s0);
         }
         __syncthreads();   // (buffer 0 of K is free)
-        for (int kt = kt0; kt < kt1; kt += 2) {
+        for (int kt = kt0; kt < kt1; kt += NB) {
             step(kt, s0, s1, 0);
             if (kt + 1 < kt1) step(kt + 1, s1, s0, 1);
+            if constexpr (NB == 4) {
+                if (kt + 2 < kt1) step(kt + 2, s0, s1, 2);
+                if (kt + 3 < kt1) step(kt + 3, s1, s0, 3);
+            }
         }
+        wait_loads<0>();   // (no load may land after the LDS is given back)
     }
 
     if (idle) return;
@@ -782,7 +814,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
 // keys of its own pairs only (8191 tokens, 8 heads of 128: 777 us with the tiles fastest, the CUs busy
 // for 0.69 of it; 594 us so).
 template <class T, int HD>
-__global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_chunk(PagedAttn a) {
+__global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_chunk(PagedAttn a) {
     __shared__ __align__(16) ChunkLds<HD> lds;
     const int pairs = a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
     const int kvh = pair % a.kv.n_kv, b = pair / a.kv.n_kv;
@@ -904,7 +936,6 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         if (t0 == 0 && tid == 0) a.bal_tiles[kvh * tiles + e] = BalTile{first, num, b, rt};
         chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first + t0, sp.first + t1, part, lds);
         u += t1 - t0;
-        __syncthreads();   // (the next row tile's loads overwrite this one's LDS)
     }
 }
 
@@ -1013,7 +1044,7 @@ __global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
 // How a call is cut: a function of its arguments alone (the workspace's size follows from it)
 struct Plan {
     bool few, chunk;
-    int few_qt, few_tiles, few_split;
+    int few_qt, few_waves, few_tiles, few_split;
     int chunk_tiles;       // row tiles of the longest sequence
     int balanced_tiles;    // 0: one row tile per workgroup; else the most row tiles that there can be per head
 };
@@ -1029,7 +1060,12 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
         const int64_t most = rows < FEW_ROWS ? rows : FEW_ROWS;
         p.few_qt = most <= 16 || (p.chunk && group <= 16) ? 1 : 2;
         p.few_tiles = (int) ((most + 16 * p.few_qt - 1) / (16 * p.few_qt));
-        const int64_t n = std::min((1024 + (int64_t) B * n_kv - 1) / ((int64_t) B * n_kv), max_keys / 256);
+        // Splits up to about 16 waves per CU. Alone: workgroups of 8 waves where they do not outnumber
+        // the CUs, splits of at least 2048 keys (fewer are through before a second launch has joined
+        // them). Beside chunks, of sequences whose number is not known: of 4 waves and 256 keys.
+        const int64_t pairs = (int64_t) B * n_kv;
+        p.few_waves = !p.chunk && pairs * p.few_tiles <= 256 ? 8 : 4;
+        const int64_t n = std::min((4096 + p.few_waves * pairs - 1) / (p.few_waves * pairs), max_keys / (p.chunk ? 256 : 2048));
         p.few_split = (int) std::max<int64_t>(1, std::min<int64_t>(n, 64));
     }
     if (p.chunk) {
@@ -1071,8 +1107,11 @@ void launch_attn(PagedAttn a, const Plan & p, void * ws, hipStream_t st) {
         a.part_o = (float *) ws;
         a.part_ml = a.part_o + (size_t) p.few_split * a.kv.tokens * a.group * nkv * HD;
         const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
-        if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1>), grid, dim3(FEW_WAVES * 64), 0, st, a);
-        else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2>), grid, dim3(FEW_WAVES * 64), 0, st, a);
+        const dim3 block((unsigned) p.few_waves * 64);
+        if (p.few_qt == 1 && p.few_waves == 4) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1, 4>), grid, block, 0, st, a);
+        else if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1, 8>), grid, block, 0, st, a);
+        else if (p.few_waves == 4) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2, 4>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2, 8>), grid, block, 0, st, a);
         constexpr int R = 256 / (HD / 8);
         const int rows = (int) std::min<int64_t>((int64_t) a.max_new * a.group, FEW_ROWS);
         if (a.nsplit > 4)

@@ -431,17 +431,21 @@ class PagedKV:
 
 def _paged_stream(kv, stream, what):
     """The stream of a call (torch's current one by default), on the cache's device."""
-    import torch
-    if torch.cuda.current_device() != kv.device:
+    if _torch_cuda is None:
+        _load_torch()
+    if _torch_cuda[0]() != kv.device:
         raise ValueError(f"{what}: the cache is on device {kv.device}, which is not the current one")
-    return _raw_stream(kv.device) if stream is None else stream
+    return _torch_cuda[1](kv.device) if stream is None else stream
 
 
-def _raw_stream(device):
-    """Handle of torch's current stream on device number `device`."""
+_torch_cuda = None   # torch's current device, and the handle of its current stream on a device
+
+
+def _load_torch():
+    global _torch_cuda
     import torch
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the stream object costs 3 us more)
-    return raw(device) if raw is not None else torch.cuda.current_stream(device).cuda_stream
+    _torch_cuda = (torch.cuda.current_device, raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
 
 
 def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=False, pos=None, n_bad=None,
@@ -484,7 +488,8 @@ def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys, window=0) -> i
 def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0, prefix=None, ws=None, stream=None):
     """Attention of the new tokens q [T][nh][hd] over the pages of `kv` (PagedKV) into out [T][nh][hd]
     (include/gsvk.h gsvk_op_attn_paged); lse [T][nh] fp32, prefix [B] int32. ws None: a workspace from
-    torch's allocator, which belongs to torch's current stream."""
+    torch's allocator (on torch's current stream only: another stream's call brings its own, of
+    attn_paged_workspace_bytes)."""
     dev, st = kv.device, _paged_stream(kv, stream, "attn_paged")
     sh = q.shape
     if len(sh) != 3 or out.shape != sh or q.dtype != kv.dtype:
@@ -498,11 +503,11 @@ def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0,
         max_keys = kv.cols * kv.page_size
     wp, wn = None, 0
     if ws is None:
+        if stream is not None and stream != _torch_cuda[1](dev):
+            raise ValueError("attn_paged: a stream other than torch's current one needs a ws of its own")
         wn = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys, window)
         if wn:
             import torch
-            if stream is not None and stream != _raw_stream(dev):
-                raise ValueError("attn_paged: a stream other than torch's current one needs a ws of its own")
             ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
             wp = ws.data_ptr()
     elif ws.get_device() != dev or not ws.is_contiguous():
