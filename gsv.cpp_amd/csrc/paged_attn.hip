@@ -16,7 +16,7 @@
 //                       maximum and sum; K goes straight into the operand registers
 //                       (v_mfma_f32_16x16x32: 16 keys x 32 dims), V through a tile of LDS that
 //                       belongs to the wave, so the loop has no barrier. Bound by HBM.
-//   k_attn_paged_chunk  longer chunks: 8 waves of 32 rows share key tiles of 64 in LDS (double
+//   k_attn_paged_chunk  longer chunks: 4 waves of 32 rows share key tiles of 64 in LDS (double
 //                       buffered), v_mfma_f32_32x32x16.
 // Where that makes too few workgroups, or too unequal ones, keys are divided too: k_attn_paged_few cuts
 // each row tile into nsplit runs of keys, k_attn_paged_balanced all row tiles together into equal
@@ -52,7 +52,7 @@ typedef const __attribute__((address_space(4))) int32_t pg_table;   // (no store
 
 constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
 constexpr int FEW_KEYS = 32;
-constexpr int CH_WAVES = 8, CH_KEYS = 64, CH_ROWS = CH_WAVES * 32;
+constexpr int CH_WAVES = 4, CH_KEYS = 64, CH_ROWS = CH_WAVES * 32;
 constexpr float M_NONE = -FLT_MAX;    // m of a row that has seen nothing: exp2(score - m) of -inf is 0
 constexpr float M_ROOM = 12.0f, M_SET = 4.0f;
 
@@ -461,12 +461,10 @@ __device__ __forceinline__ void load_lds(const char * base, uint32_t off, uint16
                  : "memory");
 #endif
 }
-// All but the last N loads of this wave have landed, every LDS operation of it is done (gfx9
-// encoding: vmcnt in bits 3:0 and 15:14, lgkmcnt in 11:8, expcnt not waited on); then all waves' are.
-// In order: other loads of the wave, before or after these, only make it wait longer.
-template <int N>
+// Every load of this wave has landed, every LDS operation of it is done (gfx9 encoding: vmcnt in bits
+// 3:0 and 15:14, lgkmcnt in 11:8, expcnt not waited on); then all waves' are.
 __device__ __forceinline__ void wait_loads() {
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
+    __builtin_amdgcn_s_waitcnt(0x7 << 4);
 #ifdef GSVK_HOSTEMU
     __syncthreads();
 #else
@@ -476,11 +474,9 @@ __device__ __forceinline__ void wait_loads() {
 
 // LDS of a workgroup
 template <int HD>
-constexpr int ch_ahead() { return HD == 128 ? 1 : 3; }   // tiles of V in flight beyond the current one (K: one more)
-template <int HD>
 struct ChunkLds {
-    uint16_t k[ch_ahead<HD>() + 1][CH_KEYS * HD];
-    uint16_t v[ch_ahead<HD>() + 1][CH_KEYS * HD];
+    uint16_t k[2][CH_KEYS * HD];
+    uint16_t v[2][CH_KEYS * HD];
     int flag[2];   // [0] a table entry names no page; [1] tile + 1 that holds infinities or NaNs
 };
 
@@ -504,9 +500,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
                                            float * part, ChunkLds<HD> & lds) {
     constexpr int C = HD / 8, NT = CH_WAVES * 64;
     constexpr int NK = HD / 16, DT = HD / 32;
-    constexpr int NL = C >= CH_WAVES ? C / CH_WAVES : 1;   // direct loads of a wave per tile of K (and of V)
-    constexpr int AHEAD = ch_ahead<HD>(), NB = AHEAD + 1;
-    constexpr int FLY = (HD > 32 ? 2 : 1) * NL * (AHEAD - 1);   // a wave's loads that a step leaves in flight
+    constexpr int NL = C / CH_WAVES;   // direct loads of a wave per tile of K (and of V)
     auto & s_k = lds.k;
     auto & s_v = lds.v;
     auto & s_flag = lds.flag;
@@ -535,18 +529,19 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
     }
     pg_table * tb = (pg_table *) (a.kv.table + b * a.kv.table_stride);
 
-    // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (8 j + wave) * 64 on
-    // (all within one group of 16 keys, one page); with 32 dims waves 0-3 load K, 4-7 V.
+    // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (j CH_WAVES + wave) * 64 on,
+    // all within one group of 16 keys, so within one page.
+    const auto piece = [&](int j) { return j * CH_WAVES + wave; };
     uint32_t off_k[NL], off_v[NL];
 #pragma unroll
     for (int j = 0; j < NL; j++) {
-        const int u = ((j * CH_WAVES + wave) % C) * 64 + lane, key = u / C;
+        const int u = piece(j) * 64 + lane, key = u / C;
         off_k[j] = ((key & 15) * HD + (((u % C) ^ swz_k<HD>(key)) << 3)) * 2;
         off_v[j] = ((key & 15) * HD + (((u % C) ^ swz_vc<HD>(key)) << 3)) * 2;
     }
     // pages of the wave's key groups in tile kt (past the last tile: that tile's), and their byte offsets
     const auto group_of = [&](int kt, int j) {
-        return min(kt, kt1 - 1) * CH_KEYS + ((j * CH_WAVES + wave) % C) * (CH_KEYS / C) / 16 * 16;
+        return min(kt, kt1 - 1) * CH_KEYS + piece(j) * (CH_KEYS / C) / 16 * 16;
     };
     const auto pages = [&](int kt, int (&pg)[NL]) {
 #pragma unroll
@@ -560,14 +555,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
     int64_t at_v[NL] = {};   // offsets of the tile whose V comes next
     const auto load = [&](const uint16_t * cache, const int64_t (&at)[NL], const uint32_t (&off)[NL], uint16_t * lds) {
 #pragma unroll
-        for (int j = 0; j < NL; j++)
-            load_lds(reinterpret_cast<const char *>(cache) + at[j], off[j], lds + ((j * CH_WAVES + wave) % C) * 512);
-    };
-    const auto load_k = [&](const int64_t (&at)[NL], int buf) {
-        if (HD > 32 || wave < 4) load(a.kv.k, at, off_k, s_k[buf]);
-    };
-    const auto load_v = [&](const int64_t (&at)[NL], int buf) {
-        if (HD > 32 || wave >= 4) load(a.kv.v, at, off_v, s_v[buf]);
+        for (int j = 0; j < NL; j++) load_lds(reinterpret_cast<const char *>(cache) + at[j], off[j], lds + piece(j) * 512);
     };
 
     float m = M_NONE, l = 0.0f;
@@ -661,13 +649,12 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             }
             __syncthreads();
         }
-        // V of tile kt + AHEAD, K of the one after it, into the buffers that step kt - 1 read. Past the last tile
-        // nothing (AHEAD 1), or the last one again: the count of loads in flight stays the same.
-        if (AHEAD > 1 || kt + AHEAD < kt1) load_v(at_v, (buf + AHEAD) % NB);
-        if (AHEAD > 1 || kt + AHEAD + 1 < kt1) {
-            offsets(kt + AHEAD + 1, pg_n, at_v);
-            load_k(at_v, buf);
-            pages(kt + AHEAD + 2, pg_n);
+        // V of the next tile, K of the one after it, into the buffers that the last step read
+        if (kt + 1 < kt1) load(a.kv.v, at_v, off_v, s_v[buf ^ 1]);
+        if (kt + 2 < kt1) {
+            offsets(kt + 2, pg_n, at_v);
+            load(a.kv.k, at_v, off_k, s_k[buf]);
+            pages(kt + 3, pg_n);
         }
         if (kb < whi && kb + 2 * CH_KEYS > wlo) {   // a row of the wave sees this tile, or the next one
             top *= a.scale_log2;
@@ -683,10 +670,10 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             }
             uint4 kf[2][NK / 2];
             typename T::v8 vf[2][DT], pf;
-            read_k(kf[0], (buf + 1) % NB, 0);
+            read_k(kf[0], buf ^ 1, 0);
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                if (q < 3) read_k(kf[(q + 1) & 1], (buf + 1) % NB, q + 1);
+                if (q < 3) read_k(kf[(q + 1) & 1], buf ^ 1, q + 1);
                 read_v(vf[q & 1], buf, q);
                 mul_k(sn, kf[q & 1], q);
                 if (q > 0) {
@@ -734,78 +721,86 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             if (!(kb + CH_KEYS >= wlo_max && kb + 2 * CH_KEYS <= whi_min && !has_bad)) mask(sn, kt + 1);
             top = top_of(sn);
         }
-        wait_loads<FLY>();   // V of the next tile and K of the one after it are there
+        wait_loads();   // V of the next tile and K of the one after it are there
     };
 
-    if (kt0 < kt1) {
+    {
         if (tid < 2) s_flag[tid] = 0;
-        __syncthreads();
+        int pg[NL], pg2[NL];
+        pages(kt0, pg);
+        pages(kt0 + 1, pg2);
+        pages(kt0 + 2, pg_n);
+        offsets(kt0, pg, at_v);
+        load(a.kv.k, at_v, off_k, s_k[0]);
+        load(a.kv.v, at_v, off_v, s_v[0]);
+        offsets(kt0 + 1, pg2, at_v);
+        load(a.kv.k, at_v, off_k, s_k[1]);   // (of a single tile: the same again)
         // table entries that name no page: rare, and every tile then takes its masks
+        bool bad = false;
         const int c0 = (kt0 * CH_KEYS) >> a.kv.page_shift, c1 = (min(kt1 * CH_KEYS, khi) - 1) >> a.kv.page_shift;
-        for (int c = c0 + tid; c <= c1; c += NT)
-            if (page_of(a, tb, c << a.kv.page_shift) < 0) s_flag[0] = 1;
-        int pg[NB][NL];
-#pragma unroll
-        for (int i = 0; i < NB; i++) pages(kt0 + i, pg[i]);
-        pages(kt0 + NB, pg_n);
-        offsets(kt0, pg[0], at_v);
-        load_k(at_v, 0);
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            load_v(at_v, i);
-            offsets(kt0 + i + 1, pg[i + 1], at_v);
-            load_k(at_v, i + 1);
-        }
-        wait_loads<FLY>();
-        has_bad = __builtin_amdgcn_readfirstlane(s_flag[0]) != 0;
+        for (int c = c0 + tid; c <= c1; c += NT) bad |= page_of(a, tb, c << a.kv.page_shift) < 0;
+        wait_loads();
+        if (bad) s_flag[0] = 1;
         // (a wave whose rows see none of the first tiles passes over them: its scores are then these)
         pg_f16 s0[2], s1[2];
 #pragma unroll
         for (int v = 0; v < 16; v++) s1[0][v] = s1[1][v] = -INFINITY;
         scores(s0, 0);
+        __syncthreads();   // (the flag is set; buffer 0 of K is free)
+        has_bad = __builtin_amdgcn_readfirstlane(s_flag[0]) != 0;
         {
             const int kb = kt0 * CH_KEYS;
             if (!(kb >= wlo_max && kb + CH_KEYS <= whi_min && !has_bad)) mask(s0, kt0);
             top = top_of(s0);
         }
-        __syncthreads();   // (buffer 0 of K is free)
-        for (int kt = kt0; kt < kt1; kt += NB) {
+        for (int kt = kt0; kt < kt1; kt += 2) {
             step(kt, s0, s1, 0);
             if (kt + 1 < kt1) step(kt + 1, s1, s0, 1);
-            if constexpr (NB == 4) {
-                if (kt + 2 < kt1) step(kt + 2, s0, s1, 2);
-                if (kt + 3 < kt1) step(kt + 3, s1, s0, 3);
-            }
         }
-        wait_loads<0>();   // (no load may land after the LDS is given back)
     }
 
     if (idle) return;
     l = sum_x32(l);
-    if (rw + li >= s.rows) return;
     const int64_t row = s.row0 + tok, id = row * nh + h;
-    if (!part) {
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; d++)
-#pragma unroll
-            for (int v = 0; v < 16; v += 4) {
-                pg_f4 x = {o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]};
-                x *= inv;
-                if (l == 0.0f) x = pg_f4{0.0f, 0.0f, 0.0f, 0.0f};
-                store4<T>(a, row, h * HD + 32 * d + 2 * v + 4 * lh, x[0], x[1], x[2], x[3]);
-            }
-        if (a.lse && lh == 0) a.lse[id] = lse_of(m, l);
-    } else {
-        const int rl = wave * 32 + li;
+    const bool valid = rw + li < s.rows;
+    if (part) {
+        // in register order: 1 KB per store
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int v = 0; v < 16; v += 4)
-                *reinterpret_cast<float4 *>(part + rl * HD + 32 * d + 2 * v + 4 * lh) =
+                *reinterpret_cast<float4 *>(part + (((wave * DT + d) * 4 + v / 4) * 64 + lane) * 4) =
                     make_float4(o[d][v], o[d][v + 1], o[d][v + 2], o[d][v + 3]);
-        if (lh == 0) *reinterpret_cast<float2 *>(part + CH_ROWS * HD + 2 * rl) = make_float2(m, l);
+        if (lh == 0) *reinterpret_cast<float2 *>(part + CH_ROWS * HD + 2 * (wave * 32 + li)) = make_float2(m, l);
+        return;
     }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    const auto val = [&](int d, int v) { return l != 0.0f ? o[d][v] * inv : 0.0f; };
+    if (a.out_f32) {
+        if (valid)
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4)
+                    *reinterpret_cast<float4 *>((float *) a.out + row * a.out_stride + h * HD + 32 * d + 2 * v + 4 * lh) =
+                        make_float4(val(d, v), val(d, v + 1), val(d, v + 2), val(d, v + 3));
+    } else {
+        // The lane 32 away holds the other 4 of 8 dims: the two trade halves of two groups of 8 and store
+        // 16 bytes each.
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 8) {
+                const auto x = __builtin_amdgcn_permlane32_swap(pg_pack<T>(val(d, v), val(d, v + 1)),
+                                                                pg_pack<T>(val(d, v + 4), val(d, v + 5)), false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(pg_pack<T>(val(d, v + 2), val(d, v + 3)),
+                                                                pg_pack<T>(val(d, v + 6), val(d, v + 7)), false, false);
+                if (valid)
+                    *reinterpret_cast<uint4 *>((uint16_t *) a.out + row * a.out_stride + h * HD + 32 * d + 2 * v + 8 * lh) =
+                        make_uint4(x[0], y[0], x[1], y[1]);
+            }
+    }
+    if (a.lse && lh == 0 && valid) a.lse[id] = lse_of(m, l);
 }
 
 // One row tile per workgroup, all its keys. (head, sequence) fastest, then the row tiles from each
@@ -829,7 +824,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
 // tile, key), are cut into equal runs, one per workgroup (CUs that would wait for the longest row
 // tile share its keys). A row tile that a cut goes through is joined by k_attn_paged_join. Every workgroup computes
 // the same list of row tiles and running sums; the ids of an XCD take consecutive runs.
-constexpr int BAL_GROUPS = 256, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
+constexpr int BAL_GROUPS = 512, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
 
 struct BalHead { int tiles, run; };                 // row tiles of a head, key tiles per workgroup
 struct BalTile { int first, num, b, rt; };          // a row tile's place in its head's list of key tiles
@@ -843,7 +838,7 @@ struct BalLds {
 };
 
 // Exclusive prefix sums of x over the workgroup's threads; total to every thread. Two barriers.
-__device__ __forceinline__ int scan512(int x, int * s_wave, int & total) {
+__device__ __forceinline__ int scan_group(int x, int * s_wave, int & total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int y = x;
 #pragma unroll
@@ -881,23 +876,24 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     const int tid = threadIdx.x;
     // row tiles of the sequences
     int tiles = 0;
-    {
-        int n = 0;
-        if (tid < a.kv.B) {
-            const Seq s = seq_of(a, tid);
+    for (int b0 = 0; b0 < a.kv.B; b0 += CH_WAVES * 64) {
+        int n = 0, add = 0;
+        const int b = b0 + tid;
+        if (b < a.kv.B) {
+            const Seq s = seq_of(a, b);
             if (s.rows >= a.min_rows && s.rows <= a.max_rows) n = (s.rows + CH_ROWS - 1) / CH_ROWS;
         }
-        n = scan512(n, bal.wave, tiles);
-        if (tid < a.kv.B) bal.tiles[tid] = n;
-        if (tid == 0) bal.tiles[a.kv.B] = tiles;
-        tiles = min(tiles, BAL_TILES);   // (the plan has made sure)
-        __syncthreads();
+        n = scan_group(n, bal.wave, add);
+        if (b < a.kv.B) bal.tiles[b] = tiles + n;
+        tiles += add;
     }
+    if (tid == 0) bal.tiles[a.kv.B] = tiles;
+    __syncthreads();
+    tiles = __builtin_amdgcn_readfirstlane(min(tiles, BAL_TILES));   // (the plan has made sure)
     if (tiles == 0) {
         if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{0, 1};
         return;
     }
-    tiles = __builtin_amdgcn_readfirstlane(tiles);
     int units = 0;   // key tiles of a head
     for (int e0 = 0; e0 < tiles; e0 += CH_WAVES * 64) {
         int n = 0, add = 0;
@@ -906,7 +902,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
             const int b = last_le(bal.tiles, a.kv.B, e);
             n = span_of(a, seq_of(a, b), e - bal.tiles[b]).num;
         }
-        n = scan512(n, bal.wave, add);
+        n = scan_group(n, bal.wave, add);
         if (e < tiles) bal.units[e] = units + n;
         units += add;
     }
@@ -920,30 +916,43 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
 
     const int w = (int) (blockIdx.x % 8) * (BAL_GROUPS / 8) + (int) (blockIdx.x / 8);
     const int64_t u0 = (int64_t) w * run, u1 = min(total, u0 + run);
-    for (int64_t u = u0; u < u1;) {
-        // (all uniform; said so for the direct loads, whose base is scalar)
-        const int kvh = __builtin_amdgcn_readfirstlane((int) (u / units)), at = __builtin_amdgcn_readfirstlane((int) (u % units));
-        const int e = __builtin_amdgcn_readfirstlane(last_le(bal.units, tiles, at));
-        const int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
-        const int rt = __builtin_amdgcn_readfirstlane(e - bal.tiles[b]);
+    if (u0 >= u1) return;
+    // (the values below are uniform; said so for the direct loads, whose base is scalar)
+    int kvh = __builtin_amdgcn_readfirstlane((int) (u0 / units));
+    const int at = __builtin_amdgcn_readfirstlane((int) (u0 - (int64_t) kvh * units));
+    int e = __builtin_amdgcn_readfirstlane(last_le(bal.units, tiles, at));
+    int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
+    int left = (int) (u1 - u0), t0 = at - __builtin_amdgcn_readfirstlane(bal.units[e]);
+    Seq s = seq_of(a, b);
+    for (bool more = false;; more = true) {
         const int first = __builtin_amdgcn_readfirstlane(bal.units[e]);
-        const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first, t0 = at - first;
-        const int t1 = __builtin_amdgcn_readfirstlane((int) min((int64_t) num, t0 + (u1 - u)));
-        const Seq s = seq_of(a, b);
+        const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first, t1 = min(num, t0 + left);
+        const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
         const Span sp = span_of(a, s, rt);
         float * part = nullptr;
-        if (t1 - t0 < num) part = a.part_o + (int64_t) (2 * w + (u > u0)) * bal_slot<HD>();
+        if (t1 - t0 < num) part = a.part_o + (int64_t) (2 * w + more) * bal_slot<HD>();
         if (t0 == 0 && tid == 0) a.bal_tiles[kvh * tiles + e] = BalTile{first, num, b, rt};
         chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first + t0, sp.first + t1, part, lds);
-        u += t1 - t0;
+        left -= t1 - t0;
+        if (left == 0) break;
+        t0 = 0;
+        if (++e == tiles) {
+            e = 0;
+            kvh++;
+        }
+        const int next = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
+        if (next != b) {
+            b = next;
+            s = seq_of(a, b);
+        }
     }
 }
 
-// The row tiles that k_attn_paged_balanced has cut: workgroup = (256 / (HD / 8) rows, row tile, head), a
-// thread 8 dims of a row
+// The row tiles that k_attn_paged_balanced has cut: workgroup = (a wave's 32 rows and 32 dims, row tile,
+// head), a thread 4 dims of a row, as the wave stored them
 template <class T, int HD>
 __global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
-    constexpr int C = HD / 8, R = 256 / C;
+    constexpr int DT = HD / 32;
     const BalHead hd = *a.bal_head;
     const int e = blockIdx.y, kvh = blockIdx.z;
     if (e >= hd.tiles) return;
@@ -951,30 +960,29 @@ __global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
     // (a head's key tiles follow the last head's)
     const BalTile last = a.bal_tiles[hd.tiles - 1];
     const int64_t u0 = (int64_t) kvh * (last.first + last.num) + t.first, u1 = u0 + t.num;
-    const int64_t w0 = u0 / hd.run, w1 = (u1 - 1) / hd.run;
+    const int w0 = (int) (u0 / hd.run), w1 = (int) ((u1 - 1) / hd.run);
     if (w0 == w1) return;
     const Seq s = seq_of(a, t.b);
-    const int rl = blockIdx.x * R + threadIdx.x / C, col = (threadIdx.x % C) * 8, r = t.rt * CH_ROWS + rl;
+    const int lane = threadIdx.x & 63, vq = threadIdx.x >> 6;
+    const int rl = (int) (blockIdx.x / DT) * 32 + (lane & 31), r = t.rt * CH_ROWS + rl;
     if (r >= s.rows) return;
-    float M = M_NONE, L = 0.0f, x[8] = {};
-    for (int64_t w = w0; w <= w1; w++) {
-        const float * part = a.part_o + (2 * w + (w * hd.run < u0)) * bal_slot<HD>();
+    const bool late = (int64_t) w0 * hd.run < u0;   // the first part is not its workgroup's first
+    float M = M_NONE, L = 0.0f, x[4] = {};
+    for (int w = w0; w <= w1; w++) {
+        const float * part = a.part_o + (2 * (int64_t) w + (w == w0 && late)) * bal_slot<HD>();
         const float2 ml = *reinterpret_cast<const float2 *>(part + CH_ROWS * HD + 2 * rl);
-        const float4 * p = reinterpret_cast<const float4 *>(part + rl * HD + col);
-        const float4 u = p[0], v = p[1];
+        const float4 u = *reinterpret_cast<const float4 *>(part + ((blockIdx.x * 4 + vq) * 64 + lane) * 4);
         const float mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml.x - mn);
         M = mn;
         L = __builtin_fmaf(L, c, ml.y * f);
         x[0] = __builtin_fmaf(x[0], c, u.x * f); x[1] = __builtin_fmaf(x[1], c, u.y * f);
         x[2] = __builtin_fmaf(x[2], c, u.z * f); x[3] = __builtin_fmaf(x[3], c, u.w * f);
-        x[4] = __builtin_fmaf(x[4], c, v.x * f); x[5] = __builtin_fmaf(x[5], c, v.y * f);
-        x[6] = __builtin_fmaf(x[6], c, v.z * f); x[7] = __builtin_fmaf(x[7], c, v.w * f);
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
-    const int tok = r / a.group, h = kvh * a.group + r % a.group;
-    store8<T>(a, s.row0 + tok, h * HD + col, x);
+    for (int i = 0; i < 4; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
+    const int tok = r / a.group, h = kvh * a.group + r % a.group, col = 32 * (int) (blockIdx.x % DT) + 8 * vq + 4 * (lane >> 5);
+    store4<T>(a, s.row0 + tok, h * HD + col, x[0], x[1], x[2], x[3]);
     if (a.lse && col == 0) a.lse[(s.row0 + tok) * a.group * a.kv.n_kv + h] = lse_of(M, L);
 }
 
@@ -1072,7 +1080,7 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
         p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);
         // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence
         const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS), most = tokens * group / CH_ROWS + B;
-        const bool enough = least * n_kv >= 768 || (least * n_kv >= 192 && max_keys <= 1024) || max_keys <= 256;
+        const bool enough = least * n_kv >= 1536 || max_keys <= 1024;
         if (!enough && B <= BAL_SEQS && most <= BAL_TILES) p.balanced_tiles = (int) most;
     }
     return p;
@@ -1094,7 +1102,7 @@ void launch_attn(PagedAttn a, const Plan & p, void * ws, hipStream_t st) {
             a.bal_tiles = (BalTile *) (a.bal_head + 1);
             a.part_o = (float *) ((char *) ws + bal_tables(p, a.kv.n_kv));
             hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), dim3(BAL_GROUPS), dim3(CH_WAVES * 64), 0, st, a);
-            hipLaunchKernelGGL((k_attn_paged_join<T, HD>), dim3(CH_ROWS / (256 / (HD / 8)), (unsigned) p.balanced_tiles, nkv),
+            hipLaunchKernelGGL((k_attn_paged_join<T, HD>), dim3(CH_WAVES * (HD / 32), (unsigned) p.balanced_tiles, nkv),
                                dim3(256), 0, st, a);
         } else {
             hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) p.chunk_tiles * nkv * B), dim3(CH_WAVES * 64), 0, st, a);
