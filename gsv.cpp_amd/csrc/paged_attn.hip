@@ -20,7 +20,7 @@
 //                       buffered), v_mfma_f32_32x32x16.
 // Where that makes too few workgroups, or too unequal ones, keys are divided too: k_attn_paged_few cuts
 // each row tile into nsplit runs of keys, k_attn_paged_balanced all row tiles together into equal
-// runs; (maximum, sum, unnormalised output) of the parts are joined by k_attn_paged_merge and _join.
+// runs; (maximum, sum, unnormalised output) of the parts are joined by k_attn_paged_join.
 //
 // Softmax. Exponents are base 2. The reference exponent m of a row is not its running maximum but
 // follows it: it is moved (and O, l rescaled) only when a score exceeds it by more than 2^12, to
@@ -69,16 +69,19 @@ struct PagedAttn {
     const int32_t * prefix;
     float * part_o;     // [nsplit][tokens * nh][HD]
     float * part_ml;    // [nsplit][tokens * nh][2]
-    BalHead * bal_head;   // k_attn_paged_balanced's (part_o: its slots)
+    BalHead * bal_head;   // k_attn_paged_balanced's tables and slots
     BalTile * bal_tiles;
+    float * bal_part;
     float scale_log2;
     int group;   // query heads per key/value head
     int window;
     int max_new;
     int out_f32;
-    int nsplit;       // of this launch
-    int min_rows;     // sequences of fewer rows are another launch's
-    int max_rows;     // and of more
+    int nsplit;         // runs that a sequence of few rows is cut into
+    int min_rows;       // of a chunk: sequences of fewer rows are few_tile's
+    int chunk_groups;   // workgroups of chunks
+    int bal_most;       // row tiles of a head that there can be, if balanced
+    int few_rows;       // rows that a sequence of few rows can have
 };
 
 template <class T>
@@ -216,21 +219,30 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 
 // ---- few rows ------------------------------------------------------------------------------------
 
-// QT tiles of 16 rows per workgroup of NW waves
-template <class T, int HD, int QT, int NW>
-__global__ void __launch_bounds__(NW * 64) k_attn_paged_few(PagedAttn a) {
-    constexpr int C = HD / 8, NV = FEW_KEYS * C / 64, NK = HD / 32, DT = HD / 16, OS = HD + 4;
-    constexpr int VB = FEW_KEYS * HD * 2, OB = 16 * OS * 4;   // LDS bytes of a wave: V tile, outputs
-    __shared__ __align__(16) char s_mem[NW * (VB > OB ? VB : OB)];
-    __shared__ float s_ml[NW][QT * 16][2];
+// LDS of a wave (V tile, then outputs) and of a workgroup
+template <int HD>
+constexpr int few_wave_lds() { return FEW_KEYS * HD * 2 > 16 * (HD + 4) * 4 ? FEW_KEYS * HD * 2 : 16 * (HD + 4) * 4; }
+template <int HD, int QT, int NW>
+struct FewLds {
+    char mem[NW * few_wave_lds<HD>()];
+    float ml[NW][QT * 16][2];
+};
 
-    const int b = blockIdx.z, kvh = blockIdx.y;
-    const int split = blockIdx.x % a.nsplit, rt = blockIdx.x / a.nsplit;
+// QT tiles of 16 rows of (head kvh, sequence b) from row tile rt on, keys of one of nsplit runs, by a
+// workgroup of NW waves
+template <class T, int HD, int QT, int NW>
+__device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, int rt, int split, int min_rows,
+                                         int max_rows, FewLds<HD, QT, NW> & lds) {
+    constexpr int C = HD / 8, NV = FEW_KEYS * C / 64, NK = HD / 32, DT = HD / 16, OS = HD + 4;
+    constexpr int VB = few_wave_lds<HD>();
+    char * s_mem = lds.mem;
+    auto & s_ml = lds.ml;
+
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq s = seq_of(a, b);
     const int r0 = rt * QT * 16;
-    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    if (r0 >= s.rows || s.rows < min_rows || s.rows > max_rows) return;
     const int nh = a.group * a.kv.n_kv;
     const int tok0 = r0 / a.group, tok1 = min(r0 + QT * 16, s.rows) - 1, tokl = tok1 / a.group;
     const int klo = key_lo(a, s, tok0), khi = key_hi(s, tokl);
@@ -443,6 +455,13 @@ __global__ void __launch_bounds__(NW * 64) k_attn_paged_few(PagedAttn a) {
             }
         }
     }
+}
+
+// Calls whose sequences all have few rows
+template <class T, int HD, int QT, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) k_attn_paged_few(PagedAttn a) {
+    __shared__ __align__(16) FewLds<HD, QT, NW> lds;
+    few_tile<T, HD, QT, NW>(a, blockIdx.z, blockIdx.y, blockIdx.x / a.nsplit, blockIdx.x % a.nsplit, 1, FEW_ROWS, lds);
 }
 
 // ---- chunks ----------------------------------------------------------------------------------------
@@ -803,6 +822,19 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
     if (a.lse && lh == 0 && valid) a.lse[id] = lse_of(m, l);
 }
 
+// What a launch of chunks holds in LDS: a workgroup past the first a.chunk_groups takes the sequences
+// of few rows that stand beside the chunks (no launch of their own: 10 us of a small mixed call).
+template <int HD>
+union MixLds {
+    ChunkLds<HD> chunk;
+    FewLds<HD, 2, CH_WAVES> few;
+};
+template <class T, int HD>
+__device__ __forceinline__ void few_beside(const PagedAttn & a, MixLds<HD> & lds) {
+    const int f = (int) blockIdx.x - a.chunk_groups, split = f % a.nsplit, kvh = f / a.nsplit % a.kv.n_kv;
+    few_tile<T, HD, 2, CH_WAVES>(a, f / a.nsplit / a.kv.n_kv, kvh, 0, split, 1, FEW_ROWS, lds.few);
+}
+
 // One row tile per workgroup, all its keys. (head, sequence) fastest, then the row tiles from each
 // sequence's last, which sees the most keys, to its first: the longest workgroups start first on
 // every XCD (ids go round-robin to the 8 XCDs), and with pairs a multiple of 8 an XCD's L2 holds the
@@ -810,14 +842,18 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
 // for 0.69 of it; 594 us so).
 template <class T, int HD>
 __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_chunk(PagedAttn a) {
-    __shared__ __align__(16) ChunkLds<HD> lds;
+    __shared__ __align__(16) MixLds<HD> lds;
+    if ((int) blockIdx.x >= a.chunk_groups) {
+        few_beside<T, HD>(a, lds);
+        return;
+    }
     const int pairs = a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
     const int kvh = pair % a.kv.n_kv, b = pair / a.kv.n_kv;
     const Seq s = seq_of(a, b);
     const int rt = (s.rows + CH_ROWS - 1) / CH_ROWS - 1 - (int) (blockIdx.x / pairs);
-    if (rt < 0 || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    if (rt < 0 || s.rows < a.min_rows) return;
     const Span sp = span_of(a, s, rt);
-    chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds);
+    chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds.chunk);
 }
 
 // Few row tiles of unequal length: the key tiles of all of them, in the order (head, sequence, row
@@ -871,8 +907,12 @@ __device__ __forceinline__ int last_le(const int * p, int n, int x) {
 
 template <class T, int HD>
 __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedAttn a) {
-    __shared__ __align__(16) ChunkLds<HD> lds;
+    __shared__ __align__(16) MixLds<HD> lds;
     __shared__ BalLds bal;
+    if ((int) blockIdx.x >= a.chunk_groups) {
+        few_beside<T, HD>(a, lds);
+        return;
+    }
     const int tid = threadIdx.x;
     // row tiles of the sequences
     int tiles = 0;
@@ -881,7 +921,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         const int b = b0 + tid;
         if (b < a.kv.B) {
             const Seq s = seq_of(a, b);
-            if (s.rows >= a.min_rows && s.rows <= a.max_rows) n = (s.rows + CH_ROWS - 1) / CH_ROWS;
+            if (s.rows >= a.min_rows) n = (s.rows + CH_ROWS - 1) / CH_ROWS;
         }
         n = scan_group(n, bal.wave, add);
         if (b < a.kv.B) bal.tiles[b] = tiles + n;
@@ -930,9 +970,9 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
         const Span sp = span_of(a, s, rt);
         float * part = nullptr;
-        if (t1 - t0 < num) part = a.part_o + (int64_t) (2 * w + more) * bal_slot<HD>();
+        if (t1 - t0 < num) part = a.bal_part + (int64_t) (2 * w + more) * bal_slot<HD>();
         if (t0 == 0 && tid == 0) a.bal_tiles[kvh * tiles + e] = BalTile{first, num, b, rt};
-        chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first + t0, sp.first + t1, part, lds);
+        chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first + t0, sp.first + t1, part, lds.chunk);
         left -= t1 - t0;
         if (left == 0) break;
         t0 = 0;
@@ -948,13 +988,12 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     }
 }
 
-// The row tiles that k_attn_paged_balanced has cut: workgroup = (a wave's 32 rows and 32 dims, row tile,
-// head), a thread 4 dims of a row, as the wave stored them
+// A row tile e of head kvh, if k_attn_paged_balanced has cut it: part x of it (a wave's 32 rows and 32
+// dims), a thread 4 dims of a row, as the wave stored them
 template <class T, int HD>
-__global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
+__device__ __forceinline__ void join_tile(const PagedAttn & a, int e, int kvh, int x0) {
     constexpr int DT = HD / 32;
     const BalHead hd = *a.bal_head;
-    const int e = blockIdx.y, kvh = blockIdx.z;
     if (e >= hd.tiles) return;
     const BalTile t = a.bal_tiles[kvh * hd.tiles + e];
     // (a head's key tiles follow the last head's)
@@ -964,14 +1003,14 @@ __global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
     if (w0 == w1) return;
     const Seq s = seq_of(a, t.b);
     const int lane = threadIdx.x & 63, vq = threadIdx.x >> 6;
-    const int rl = (int) (blockIdx.x / DT) * 32 + (lane & 31), r = t.rt * CH_ROWS + rl;
+    const int rl = x0 / DT * 32 + (lane & 31), r = t.rt * CH_ROWS + rl;
     if (r >= s.rows) return;
     const bool late = (int64_t) w0 * hd.run < u0;   // the first part is not its workgroup's first
     float M = M_NONE, L = 0.0f, x[4] = {};
     for (int w = w0; w <= w1; w++) {
-        const float * part = a.part_o + (2 * (int64_t) w + (w == w0 && late)) * bal_slot<HD>();
+        const float * part = a.bal_part + (2 * (int64_t) w + (w == w0 && late)) * bal_slot<HD>();
         const float2 ml = *reinterpret_cast<const float2 *>(part + CH_ROWS * HD + 2 * rl);
-        const float4 u = *reinterpret_cast<const float4 *>(part + ((blockIdx.x * 4 + vq) * 64 + lane) * 4);
+        const float4 u = *reinterpret_cast<const float4 *>(part + ((x0 * 4 + vq) * 64 + lane) * 4);
         const float mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml.x - mn);
         M = mn;
         L = __builtin_fmaf(L, c, ml.y * f);
@@ -981,26 +1020,30 @@ __global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; i++) x[i] = L != 0.0f ? x[i] * inv : 0.0f;
-    const int tok = r / a.group, h = kvh * a.group + r % a.group, col = 32 * (int) (blockIdx.x % DT) + 8 * vq + 4 * (lane >> 5);
+    const int tok = r / a.group, h = kvh * a.group + r % a.group, col = x0 % DT * 32 + 8 * vq + 4 * (lane >> 5);
     store4<T>(a, s.row0 + tok, h * HD + col, x[0], x[1], x[2], x[3]);
     if (a.lse && col == 0) a.lse[(s.row0 + tok) * a.group * a.kv.n_kv + h] = lse_of(M, L);
 }
 
 // ---- joining the splits ------------------------------------------------------------------------------
 
-// A workgroup takes 256 / (HD / 8) / SL rows of one (sequence, head); a row's splits are dealt to SL
-// groups of HD / 8 threads, which hold 8 dims each, and the groups are joined through LDS. SL 16
-// where there are more than 4 splits (64 splits of 2 x 64 rows of 128: 54.7 us with SL 1, one split
-// after another).
+// A workgroup takes 256 / (HD / 8) / SL rows of (head kvh, sequence b), the x0-th such group; a row's
+// splits are dealt to SL groups of HD / 8 threads, which hold 8 dims each, and the groups are joined
+// through LDS. SL 16 where there are more than 4 splits (64 splits of 2 x 64 rows of 128: 54.7 us with SL 1,
+// one split after another; 5.6 us so).
+template <int HD, int SL>
+struct MergeLds {
+    float x[256 / (HD / 8) / SL][SL][HD + 4];
+    float ml[256 / (HD / 8) / SL][SL][2];
+};
 template <class T, int HD, int SL>
-__global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
+__device__ __forceinline__ void merge_rows(const PagedAttn & a, int b, int kvh, int x0, MergeLds<HD, SL> & lds) {
     constexpr int C = HD / 8, R = 256 / C / SL;
-    __shared__ float s_x[R][SL][HD + 4];
-    __shared__ float s_ml[R][SL][2];
-    const int b = blockIdx.z, kvh = blockIdx.y;
+    auto & s_x = lds.x;
+    auto & s_ml = lds.ml;
     const Seq s = seq_of(a, b);
-    const int r0 = blockIdx.x * R;
-    if (r0 >= s.rows || s.rows < a.min_rows || s.rows > a.max_rows) return;
+    const int r0 = x0 * R;
+    if (r0 >= s.rows || s.rows > FEW_ROWS) return;
     const int rr = threadIdx.x / (C * SL), sl = threadIdx.x / C % SL, col = (threadIdx.x % C) * 8;
     const int r = min(r0 + rr, s.rows - 1);
     const int nh = a.group * a.kv.n_kv, tok = r / a.group, h = kvh * a.group + r % a.group;
@@ -1047,12 +1090,28 @@ __global__ void __launch_bounds__(256) k_attn_paged_merge(PagedAttn a) {
     if (a.lse && col == 0) a.lse[id] = lse_of(M, L);
 }
 
+// Joins what the launch before it has cut: first the row tiles of chunks, then the rows of few
+template <class T, int HD, int SL>
+__global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
+    __shared__ MergeLds<HD, SL> lds;
+    constexpr int X = CH_WAVES * (HD / 32), R = 256 / (HD / 8) / SL;
+    const int tiles = a.bal_most * a.kv.n_kv * X;
+    int i = blockIdx.x;
+    if (i < tiles) {
+        join_tile<T, HD>(a, i / X % a.bal_most, i / X / a.bal_most, i % X);
+        return;
+    }
+    i -= tiles;
+    const int per = (a.few_rows + R - 1) / R;
+    merge_rows<T, HD, SL>(a, i / per / a.kv.n_kv, i / per % a.kv.n_kv, i % per, lds);
+}
+
 // ---- the host's side -----------------------------------------------------------------------------------
 
 // How a call is cut: a function of its arguments alone (the workspace's size follows from it)
 struct Plan {
-    bool few, chunk;
-    int few_qt, few_waves, few_tiles, few_split;
+    bool few, chunk;       // sequences of few rows can be there; chunks can
+    int few_rows, few_qt, few_waves, few_tiles, few_split;
     int chunk_tiles;       // row tiles of the longest sequence
     int balanced_tiles;    // 0: one row tile per workgroup; else the most row tiles that there can be per head
 };
@@ -1065,15 +1124,15 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
     p.chunk = rows > FEW_ROWS;
     p.few = !p.chunk || (B > 1 && group <= FEW_ROWS);
     if (p.few) {
-        const int64_t most = rows < FEW_ROWS ? rows : FEW_ROWS;
-        p.few_qt = most <= 16 || (p.chunk && group <= 16) ? 1 : 2;
-        p.few_tiles = (int) ((most + 16 * p.few_qt - 1) / (16 * p.few_qt));
-        // Splits up to about 16 waves per CU. Alone: workgroups of 8 waves where they do not outnumber
-        // the CUs, splits of at least 2048 keys (fewer are through before a second launch has joined
-        // them). Beside chunks, of sequences whose number is not known: of 4 waves and 256 keys.
+        // Splits up to about 16 waves per CU. Workgroups of 8 waves where they do not outnumber the CUs,
+        // of at least 2048 keys (fewer are through before a second launch has joined them), else (and
+        // beside chunks, of sequences whose number is not known) of 4 waves and 1024 keys.
+        p.few_rows = (int) std::min<int64_t>(rows, FEW_ROWS);
+        p.few_qt = p.few_rows <= 16 && !p.chunk ? 1 : 2;
+        p.few_tiles = (p.few_rows + 16 * p.few_qt - 1) / (16 * p.few_qt);
         const int64_t pairs = (int64_t) B * n_kv;
         p.few_waves = !p.chunk && pairs * p.few_tiles <= 256 ? 8 : 4;
-        const int64_t n = std::min((4096 + p.few_waves * pairs - 1) / (p.few_waves * pairs), max_keys / (p.chunk ? 256 : 2048));
+        const int64_t n = std::min((4096 + p.few_waves * pairs - 1) / (p.few_waves * pairs), max_keys / (256 * p.few_waves));
         p.few_split = (int) std::max<int64_t>(1, std::min<int64_t>(n, 64));
     }
     if (p.chunk) {
@@ -1086,48 +1145,64 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
     return p;
 }
 
-size_t bal_tables(const Plan & p, int n_kv) {   // bytes before the slots
-    const size_t n = sizeof(BalHead) + (size_t) p.balanced_tiles * n_kv * sizeof(BalTile);
-    return (n + 255) / 256 * 256;
+// The workspace: tables and slots of k_attn_paged_balanced, then the outputs, then the (maximum, sum) of
+// the splits of few rows
+struct Space { size_t slots, few, ml, end; };
+Space space_of(const Plan & p, int64_t rows, int n_kv, int hd) {
+    Space w{};
+    if (p.balanced_tiles) {
+        w.slots = (sizeof(BalHead) + (size_t) p.balanced_tiles * n_kv * sizeof(BalTile) + 255) / 256 * 256;
+        w.few = w.slots + 2 * (size_t) BAL_GROUPS * CH_ROWS * (size_t) (hd + 2) * sizeof(float);
+    }
+    w.ml = w.end = w.few;
+    if (p.few_split > 1) {
+        w.ml = w.few + (size_t) p.few_split * (size_t) rows * (size_t) hd * sizeof(float);
+        w.end = w.ml + (size_t) p.few_split * (size_t) rows * 2 * sizeof(float);
+    }
+    return w;
+}
+
+int64_t groups_of(const Plan & p, int B, int n_kv) {   // workgroups of the first launch
+    const int64_t few = (int64_t) p.few_tiles * p.few_split * n_kv * B;
+    return (p.chunk ? (p.balanced_tiles ? BAL_GROUPS : (int64_t) p.chunk_tiles * n_kv * B) : 0) + few;
+}
+
+// rows of few rows that a workgroup of k_attn_paged_join takes, and its workgroups
+int join_rows(const Plan & p, int hd) { return 256 / (hd / 8) / (p.few_split > 4 ? 16 : 1); }
+int64_t join_groups_of(const Plan & p, int B, int n_kv, int hd) {
+    const int64_t per = p.few_split > 1 ? (p.few_rows + join_rows(p, hd) - 1) / join_rows(p, hd) : 0;
+    return (int64_t) p.balanced_tiles * n_kv * (CH_WAVES * (hd / 32)) + per * n_kv * B;
 }
 
 template <class T, int HD>
 void launch_attn(PagedAttn a, const Plan & p, void * ws, hipStream_t st) {
     const unsigned nkv = (unsigned) a.kv.n_kv, B = (unsigned) a.kv.B;
+    const Space w = space_of(p, a.kv.tokens * a.group * a.kv.n_kv, a.kv.n_kv, HD);
+    a.bal_head = (BalHead *) ws;
+    a.bal_tiles = (BalTile *) (a.bal_head + 1);
+    a.bal_part = (float *) ((char *) ws + w.slots);
+    a.part_o = (float *) ((char *) ws + w.few);
+    a.part_ml = (float *) ((char *) ws + w.ml);
+    a.nsplit = p.few ? p.few_split : 1;
+    a.few_rows = p.few_rows;
     if (p.chunk) {
         a.min_rows = p.few ? FEW_ROWS + 1 : 1;
-        a.max_rows = INT32_MAX;
-        if (p.balanced_tiles) {
-            a.bal_head = (BalHead *) ws;
-            a.bal_tiles = (BalTile *) (a.bal_head + 1);
-            a.part_o = (float *) ((char *) ws + bal_tables(p, a.kv.n_kv));
-            hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), dim3(BAL_GROUPS), dim3(CH_WAVES * 64), 0, st, a);
-            hipLaunchKernelGGL((k_attn_paged_join<T, HD>), dim3(CH_WAVES * (HD / 32), (unsigned) p.balanced_tiles, nkv),
-                               dim3(256), 0, st, a);
-        } else {
-            hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), dim3((unsigned) p.chunk_tiles * nkv * B), dim3(CH_WAVES * 64), 0, st, a);
-        }
-    }
-    if (p.few) {   // (after the chunks: their part of the workspace is free again)
-        a.nsplit = p.few_split;
-        a.min_rows = 1;
-        a.max_rows = FEW_ROWS;
-        a.part_o = (float *) ws;
-        a.part_ml = a.part_o + (size_t) p.few_split * a.kv.tokens * a.group * nkv * HD;
-        const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B);
-        const dim3 block((unsigned) p.few_waves * 64);
+        a.bal_most = p.balanced_tiles;
+        a.chunk_groups = p.balanced_tiles ? BAL_GROUPS : (int) ((int64_t) p.chunk_tiles * nkv * B);
+        const dim3 grid((unsigned) groups_of(p, a.kv.B, a.kv.n_kv)), block(CH_WAVES * 64);
+        if (p.balanced_tiles) hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), grid, block, 0, st, a);
+    } else {
+        const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B), block((unsigned) p.few_waves * 64);
         if (p.few_qt == 1 && p.few_waves == 4) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1, 4>), grid, block, 0, st, a);
         else if (p.few_qt == 1) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 1, 8>), grid, block, 0, st, a);
         else if (p.few_waves == 4) hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2, 4>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_attn_paged_few<T, HD, 2, 8>), grid, block, 0, st, a);
-        constexpr int R = 256 / (HD / 8);
-        const int rows = (int) std::min<int64_t>((int64_t) a.max_new * a.group, FEW_ROWS);
-        if (a.nsplit > 4)
-            hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 16>), dim3((unsigned) ((rows + R / 16 - 1) / (R / 16)), nkv, B),
-                               dim3(256), 0, st, a);
-        else if (a.nsplit > 1)
-            hipLaunchKernelGGL((k_attn_paged_merge<T, HD, 1>), dim3((unsigned) ((rows + R - 1) / R), nkv, B), dim3(256), 0, st, a);
     }
+    const int64_t n = join_groups_of(p, a.kv.B, a.kv.n_kv, HD);
+    if (n == 0) return;
+    if (a.nsplit <= 4) hipLaunchKernelGGL((k_attn_paged_join<T, HD, 1>), dim3((unsigned) n), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_attn_paged_join<T, HD, 16>), dim3((unsigned) n), dim3(256), 0, st, a);
 }
 
 template <class T>
@@ -1135,14 +1210,6 @@ void launch_attn(const PagedAttn & a, int hd, const Plan & p, void * ws, hipStre
     if (hd == 32) launch_attn<T, 32>(a, p, ws, st);
     else if (hd == 64) launch_attn<T, 64>(a, p, ws, st);
     else launch_attn<T, 128>(a, p, ws, st);
-}
-
-// bytes of partial results: the splits' rows x (hd outputs, maximum, sum), the cut row tiles' slots
-size_t workspace_of(const Plan & p, int64_t rows, int n_kv, int hd) {
-    size_t few = 0, bal = 0;
-    if (p.few && p.few_split > 1) few = (size_t) p.few_split * (size_t) rows * (size_t) (hd + 2) * sizeof(float);
-    if (p.balanced_tiles) bal = bal_tables(p, n_kv) + 2 * (size_t) BAL_GROUPS * CH_ROWS * (size_t) (hd + 2) * sizeof(float);
-    return few > bal ? few : bal;
 }
 
 bool attn_args(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new, int64_t max_keys) {
@@ -1159,7 +1226,7 @@ extern "C" size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int6
     if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0
         || window < 0) return 0;
     if (kv->hd != 32 && kv->hd != 64 && kv->hd != 128) return 0;
-    return workspace_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->n_kv, kv->hd);
+    return space_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->n_kv, kv->hd).end;
 }
 
 extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
@@ -1185,10 +1252,10 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
                  "attn_paged: the rows of q and out must be 16-byte aligned");
     const int group = nh / kv->n_kv;
     const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys, window);
-    const size_t need = workspace_of(p, tokens * nh, kv->n_kv, kv->hd);
+    const size_t need = space_of(p, tokens * nh, kv->n_kv, kv->hd).end;
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
-    GSVK_REQUIRE((int64_t) p.chunk_tiles * kv->n_kv * kv->B <= INT32_MAX,
+    GSVK_REQUIRE(groups_of(p, kv->B, kv->n_kv) <= INT32_MAX && join_groups_of(p, kv->B, kv->n_kv, kv->hd) <= INT32_MAX,
                  "attn_paged: too many row tiles for one launch");
     a.q = (const uint16_t *) q;
     a.q_stride = q_stride;
