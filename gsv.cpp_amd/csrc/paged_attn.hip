@@ -535,8 +535,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
     const int rw = r0 + wave * 32;
     const bool idle = rw >= s.rows;
     const int tw0 = min(rw, s.rows - 1) / a.group, tw1 = min(rw + 31, s.rows - 1) / a.group;
-    const int wlo = key_lo(a, s, tw0), wlo_max = key_lo(a, s, tw1), whi_min = key_hi(s, tw0);
-    const int whi = idle ? 0 : key_hi(s, tw1);
+    const int wlo_max = key_lo(a, s, tw1), whi_min = key_hi(s, tw0);   // (tiles between are seen whole)
     const int r = min(rw + li, s.rows - 1), tok = r / a.group, h = kvh * a.group + r % a.group;
     const int lo = key_lo(a, s, tok), hi = key_hi(s, tok);
 
@@ -668,6 +667,9 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             }
             __syncthreads();
         }
+        // (the first operands are on their way from LDS while the loads are issued)
+        uint4 kf[2][NK / 2];
+        read_k(kf[0], buf ^ 1, 0);
         // V of the next tile, K of the one after it, into the buffers that the last step read
         if (kt + 1 < kt1) load(a.kv.v, at_v, off_v, s_v[buf ^ 1]);
         if (kt + 2 < kt1) {
@@ -675,71 +677,67 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
             load(a.kv.k, at_v, off_k, s_k[buf]);
             pages(kt + 3, pg_n);
         }
-        if (kb < whi && kb + 2 * CH_KEYS > wlo) {   // a row of the wave sees this tile, or the next one
-            top *= a.scale_log2;
-            if (__any(top > m + M_ROOM)) {
-                const float mn = fmaxf(m, max_x32(top) - M_SET);
-                const float f = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= f;
+        top *= a.scale_log2;
+        if (__any(top > m + M_ROOM)) {
+            const float mn = fmaxf(m, max_x32(top) - M_SET);
+            const float f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int v = 0; v < 16; v++) o[d][v] *= f;
+        }
+        typename T::v8 vf[2][DT], pf;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (q < 3) read_k(kf[(q + 1) & 1], buf ^ 1, q + 1);
+            read_v(vf[q & 1], buf, q);
+            mul_k(sn, kf[q & 1], q);
+            if (q > 0) {
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[(q - 1) & 1][d], pf, o[d]);
+            }
+            float p[8], sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 8; v++) {
+                p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[q >> 1][8 * (q & 1) + v], a.scale_log2, -m));
+                sum += p[v];
+            }
+            l += sum;
+            asm volatile("" : "+v"(l));   // (summed here: put off, the sum would keep all 32 values live)
+            pf = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
+                                     pg_pack<T>(p[6], p[7])));
+            // one product at a time among the vector instructions: in order, a run of products
+            // would hold up the exponentials behind it
+#pragma unroll
+            for (int i = 0; i < NK / 2 + (q > 0 ? DT : 0); i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                if (q > 0) __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2 + DT), 0);
+                else __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2), 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[1][d], pf, o[d]);
+        if (s_flag[1] == kt + 1) {   // the infinities and NaNs that some of the rows see
+            for (int j = 0; j < CH_KEYS; j++) {
+                const int key = kb + j, page = page_of(a, tb, key);
+                if (page < 0 || key < klo || key >= khi) continue;
+                const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lh;
+                const bool see = key >= lo && key < hi;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int v = 0; v < 16; v++) o[d][v] *= f;
+                    for (int v = 0; v < 16; v++) {
+                        const uint16_t u = vp[32 * d + 8 * (v >> 2) + (v & 3)];
+                        if (see && is_odd<T>(u)) o[d][v] += T::up(u);
+                        if ((v & 3) == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
             }
-            uint4 kf[2][NK / 2];
-            typename T::v8 vf[2][DT], pf;
-            read_k(kf[0], buf ^ 1, 0);
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (q < 3) read_k(kf[(q + 1) & 1], buf ^ 1, q + 1);
-                read_v(vf[q & 1], buf, q);
-                mul_k(sn, kf[q & 1], q);
-                if (q > 0) {
-#pragma unroll
-                    for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[(q - 1) & 1][d], pf, o[d]);
-                }
-                float p[8], sum = 0.0f;
-#pragma unroll
-                for (int v = 0; v < 8; v++) {
-                    p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[q >> 1][8 * (q & 1) + v], a.scale_log2, -m));
-                    sum += p[v];
-                }
-                l += sum;
-                asm volatile("" : "+v"(l));   // (summed here: put off, the sum would keep all 32 values live)
-                pf = v8_of<T>(make_uint4(pg_pack<T>(p[0], p[1]), pg_pack<T>(p[2], p[3]), pg_pack<T>(p[4], p[5]),
-                                         pg_pack<T>(p[6], p[7])));
-                // one product at a time among the vector instructions: in order, a run of products
-                // would hold up the exponentials behind it
-#pragma unroll
-                for (int i = 0; i < NK / 2 + (q > 0 ? DT : 0); i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    if (q > 0) __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2 + DT), 0);
-                    else __builtin_amdgcn_sched_group_barrier(0x402, 28 / (NK / 2), 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[d] = mfma32<T>(vf[1][d], pf, o[d]);
-            if (s_flag[1] == kt + 1) {   // the infinities and NaNs that some of the rows see
-                for (int j = 0; j < CH_KEYS; j++) {
-                    const int key = kb + j, page = page_of(a, tb, key);
-                    if (page < 0 || key < klo || key >= khi) continue;
-                    const uint16_t * vp = a.kv.v + key_at<HD>(a, page, kvh, key) + 4 * lh;
-                    const bool see = key >= lo && key < hi;
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int v = 0; v < 16; v++) {
-                            const uint16_t u = vp[32 * d + 8 * (v >> 2) + (v & 3)];
-                            if (see && is_odd<T>(u)) o[d][v] += T::up(u);
-                            if ((v & 3) == 3) __builtin_amdgcn_sched_barrier(0);
-                        }
-                }
-            }
-            if (!(kb + CH_KEYS >= wlo_max && kb + 2 * CH_KEYS <= whi_min && !has_bad)) mask(sn, kt + 1);
-            top = top_of(sn);
         }
+        if (!(kb + CH_KEYS >= wlo_max && kb + 2 * CH_KEYS <= whi_min && !has_bad)) mask(sn, kt + 1);
+        top = top_of(sn);
         wait_loads();   // V of the next tile and K of the one after it are there
     };
 
@@ -760,10 +758,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
         for (int c = c0 + tid; c <= c1; c += NT) bad |= page_of(a, tb, c << a.kv.page_shift) < 0;
         wait_loads();
         if (bad) s_flag[0] = 1;
-        // (a wave whose rows see none of the first tiles passes over them: its scores are then these)
         pg_f16 s0[2], s1[2];
-#pragma unroll
-        for (int v = 0; v < 16; v++) s1[0][v] = s1[1][v] = -INFINITY;
         scores(s0, 0);
         __syncthreads();   // (the flag is set; buffer 0 of K is free)
         has_bad = __builtin_amdgcn_readfirstlane(s_flag[0]) != 0;
@@ -1116,7 +1111,23 @@ struct Plan {
     int balanced_tiles;    // 0: one row tile per workgroup; else the most row tiles that there can be per head
 };
 
-Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
+// Whether equal runs of keys pay for their lists, second segments and joins. Estimated times in us: a
+// step of 64 keys takes `step` with one workgroup on a CU and up to twice that with two, so one row tile
+// per workgroup takes the longest row tile's steps or the chip's share of all, and runs the latter and
+// a fixed cost that grows with the partial results. `all` takes the other sequences of a batch as
+// 0.7 of the longest. Measured (one row tile per workgroup / runs): 2000 tokens of 32 heads of 128 over 8
+// 54 / 88, 2000 of 16 heads of 64 35 / 42, 4000 of 16 heads of 32 54 / 67; 2 x 256 tokens over 2900 keys,
+// 32 heads of 128 over 8 72 / 52, 64 tokens over 8000 keys 160 / 40, two chunks of 900 over 4900 keys beside
+// 22 single tokens 223 / 178, 4 x 512 tokens over 8100 keys 233 / 241.
+bool balanced_pays(int B, int hd, double tiles, int max_new, int64_t max_keys) {
+    const double step = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45, load = tiles / 256;
+    const double longest = (double) max_keys / 64, mean = std::max(0.0, (double) max_keys - 0.5 * max_new) / 64;
+    const double slow = 1.1 * (1.0 + std::min(std::max(load - 1.0, 0.0), 1.0) * mean / std::max(longest, 1.0));
+    const double all = mean * tiles / 512 * 1.95 * step * (B > 1 ? 0.7 : 1.0);
+    return std::max(longest * slow * step, all) > all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
+}
+
+Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
     Plan p{};
     if (max_new > tokens) max_new = (int) tokens;
     if (window && max_keys > (int64_t) window + max_new) max_keys = (int64_t) window + max_new;   // (a row tile's)
@@ -1139,8 +1150,8 @@ Plan plan_of(int B, int n_kv, int group, int64_t tokens, int max_new, int64_t ma
         p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);
         // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence
         const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS), most = tokens * group / CH_ROWS + B;
-        const bool enough = least * n_kv >= 1536 || max_keys <= 1024;
-        if (!enough && B <= BAL_SEQS && most <= BAL_TILES) p.balanced_tiles = (int) most;
+        if (B <= BAL_SEQS && most <= BAL_TILES && balanced_pays(B, hd, (double) (least * n_kv), max_new, max_keys))
+            p.balanced_tiles = (int) most;
     }
     return p;
 }
@@ -1226,7 +1237,7 @@ extern "C" size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int6
     if (!kv || !attn_args(kv, tokens, nh, max_new, max_keys) || kv->B < 1 || tokens == 0 || max_new == 0
         || window < 0) return 0;
     if (kv->hd != 32 && kv->hd != 64 && kv->hd != 128) return 0;
-    return space_of(plan_of(kv->B, kv->n_kv, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->n_kv, kv->hd).end;
+    return space_of(plan_of(kv->B, kv->n_kv, kv->hd, nh / kv->n_kv, tokens, max_new, max_keys, window), tokens * nh, kv->n_kv, kv->hd).end;
 }
 
 extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int64_t tokens, int nh, int64_t q_stride,
@@ -1251,7 +1262,7 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
                      && out_stride % (out_type == GSVK_TYPE_F32 ? 4 : 8) == 0,
                  "attn_paged: the rows of q and out must be 16-byte aligned");
     const int group = nh / kv->n_kv;
-    const Plan p = plan_of(kv->B, kv->n_kv, group, tokens, max_new, max_keys, window);
+    const Plan p = plan_of(kv->B, kv->n_kv, kv->hd, group, tokens, max_new, max_keys, window);
     const size_t need = space_of(p, tokens * nh, kv->n_kv, kv->hd).end;
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
