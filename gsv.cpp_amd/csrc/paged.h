@@ -36,7 +36,7 @@ __device__ __forceinline__ void pg_unpack8(const uint4 & u, float (&x)[8]) {
     }
 }
 
-constexpr int PG_MAX_KEYS = INT32_MAX - 255;
+constexpr int PG_MAX_KEYS = 1 << 26;   // of a sequence (sums of key tiles over a call stay in 31 bits)
 
 // gsvk_paged_kv as the kernels take it. Everything that comes from device memory is checked where
 // it is read: row ranges are cut to [0, tokens), page numbers to the cache.
@@ -60,7 +60,7 @@ struct PagedView {
         const int64_t s = seq_start[b];
         return s < 0 ? 0 : s > tokens ? tokens : s;
     }
-    // keys of sequence b that the table has room for (sums of a key and a tile stay in 31 bits)
+    // keys of sequence b that the table has room for
     __device__ __forceinline__ int keys(int b) const {
         int64_t n = kv_len[b];
         const int64_t cap = (int64_t) table_cols << page_shift;

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(AP_THREADS) k_paged_append(PagedView kv, Appen
     const int64_t p = a.pos ? a.pos[row] : slot;
     const int64_t col = slot >> kv.page_shift;
     int64_t page = -1;
-    if (slot >= 0 && col < kv.table_cols) page = kv.table[b * kv.table_stride + col];
+    if (slot >= 0 && slot < PG_MAX_KEYS && col < kv.table_cols) page = kv.table[b * kv.table_stride + col];
     if (page < 0 || page >= kv.n_pages || (a.cos && (p < 0 || p >= a.rope_rows))) {
         if (unit == 0 && a.n_bad) atomicAdd(a.n_bad, 1);
         return;

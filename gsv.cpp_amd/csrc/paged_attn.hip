@@ -857,7 +857,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
 // the same list of row tiles and running sums; the ids of an XCD take consecutive runs.
 constexpr int BAL_GROUPS = 512, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
 
-struct BalHead { int tiles, run; };                 // row tiles of a head, key tiles per workgroup
+struct BalHead { int64_t run; int tiles, pad; };    // key tiles per workgroup, row tiles of a head
 struct BalTile { int first, num, b, rt; };          // a row tile's place in its head's list of key tiles
 template <int HD>
 constexpr size_t bal_slot() { return (size_t) CH_ROWS * (HD + 2); }   // floats
@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         const int b = b0 + tid;
         if (b < a.kv.B) {
             const Seq s = seq_of(a, b);
-            if (s.rows >= a.min_rows) n = (s.rows + CH_ROWS - 1) / CH_ROWS;
+            if (s.rows >= a.min_rows) n = min((s.rows + CH_ROWS - 1) / CH_ROWS, a.bal_most);
         }
         n = scan_group(n, bal.wave, add);
         if (b < a.kv.B) bal.tiles[b] = tiles + n;
@@ -924,9 +924,9 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     }
     if (tid == 0) bal.tiles[a.kv.B] = tiles;
     __syncthreads();
-    tiles = __builtin_amdgcn_readfirstlane(min(tiles, BAL_TILES));   // (the plan has made sure)
+    tiles = __builtin_amdgcn_readfirstlane(min(tiles, a.bal_most));   // (more only if seq_start does not ascend)
     if (tiles == 0) {
-        if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{0, 1};
+        if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{1, 0, 0};
         return;
     }
     int units = 0;   // key tiles of a head
@@ -946,22 +946,24 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     units = __builtin_amdgcn_readfirstlane(units);
     const int64_t total = (int64_t) units * a.kv.n_kv;
     const int64_t share = (total + BAL_GROUPS - 1) / BAL_GROUPS;
-    const int run = (int) max(share, (int64_t) min(BAL_LEAST, (units + tiles - 1) / tiles));
-    if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{tiles, run};
+    const int64_t run = max(share, (int64_t) min(BAL_LEAST, (units + tiles - 1) / tiles));
+    if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{run, tiles, 0};
 
     const int w = (int) (blockIdx.x % 8) * (BAL_GROUPS / 8) + (int) (blockIdx.x / 8);
-    const int64_t u0 = (int64_t) w * run, u1 = min(total, u0 + run);
+    const int64_t u0 = w * run, u1 = min(total, u0 + run);
     if (u0 >= u1) return;
     // (the values below are uniform; said so for the direct loads, whose base is scalar)
     int kvh = __builtin_amdgcn_readfirstlane((int) (u0 / units));
     const int at = __builtin_amdgcn_readfirstlane((int) (u0 - (int64_t) kvh * units));
     int e = __builtin_amdgcn_readfirstlane(last_le(bal.units, tiles, at));
     int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
-    int left = (int) (u1 - u0), t0 = at - __builtin_amdgcn_readfirstlane(bal.units[e]);
+    int64_t left = u1 - u0;
+    int t0 = at - __builtin_amdgcn_readfirstlane(bal.units[e]);
     Seq s = seq_of(a, b);
     for (bool more = false;; more = true) {
         const int first = __builtin_amdgcn_readfirstlane(bal.units[e]);
-        const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first, t1 = min(num, t0 + left);
+        const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first;
+        const int t1 = (int) min((int64_t) num, t0 + left);
         const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
         const Span sp = span_of(a, s, rt);
         float * part = nullptr;
@@ -1000,7 +1002,7 @@ __device__ __forceinline__ void join_tile(const PagedAttn & a, int e, int kvh, i
     const int lane = threadIdx.x & 63, vq = threadIdx.x >> 6;
     const int rl = x0 / DT * 32 + (lane & 31), r = t.rt * CH_ROWS + rl;
     if (r >= s.rows) return;
-    const bool late = (int64_t) w0 * hd.run < u0;   // the first part is not its workgroup's first
+    const bool late = w0 * hd.run < u0;   // the first part is not its workgroup's first
     float M = M_NONE, L = 0.0f, x[4] = {};
     for (int w = w0; w <= w1; w++) {
         const float * part = a.bal_part + (2 * (int64_t) w + (w == w0 && late)) * bal_slot<HD>();

@@ -521,8 +521,8 @@ int gsvk_op_attn_prefill(const float * qkv, int B, int S, int max_len, const int
  *                [seq_start[b], seq_start[b + 1]) of the token arrays (none is allowed). Rows from
  *                seq_start[B] on belong to no sequence: nothing is written for them.
  *  kv_len      : [B] int32: keys of sequence b, its new tokens' among them: row i of its n new
- *                rows is key kv_len[b] - n + i. Keys past table_cols * page_size (or past 2^31 - 256)
- *                do not exist. */
+ *                rows is key kv_len[b] - n + i. Keys past table_cols * page_size (or past 2^26) do
+ *                not exist. */
 typedef struct gsvk_paged_kv {
     void * k;
     void * v;

@@ -7,7 +7,8 @@
 //   paged_check hd bf16 nh nkv page window prefix f32 poison tail new:keys [new:keys ...]
 //
 // prefix: 0, or the bidirectional prefix of every sequence; poison 1: the value and key of each
-// chunk's last token are NaN, 2: one table entry in seven names no page.
+// chunk's last token are NaN, 2: one table entry in seven names no page, 3: seq_start and kv_len are not
+// what they should be (rows of several sequences, past the last row, descending; only bounds are checked).
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -120,6 +121,11 @@ int main(int argc, char ** argv) {
         for (int b = 0; b < B; b++)
             if (n[b] > 1)
                 for (int d = nh * hd; d < w; d++) qkv[(size_t) (ss[b + 1] - 1) * w + d] = NAN;
+    if (poison == 3)
+        for (int b = 0; b <= B; b++) {
+            ss[b] = b % 3 == 0 ? 0 : b % 3 == 1 ? tokens : 0x7fffffff;
+            if (b < B) len[b] = b % 4 == 3 ? -0x7fffffff : b % 4 == 2 ? 0x7fffffff : tot[b];
+        }
     gsvk_paged_kv kv{kc, vc, g_bf ? GSVK_TYPE_BF16 : GSVK_TYPE_F16, nkv, hd, page, pages, 0, table, cols, cols, B, ss, len};
     gsvk_rope rope{cs, sn, max_keys, rot, 0, nullptr};
     uint16_t * q = buf<uint16_t>((size_t) tokens * nh * hd);
@@ -129,7 +135,7 @@ int main(int argc, char ** argv) {
         std::fprintf(stderr, "%s\n", gsvk::get_error());
         return 1;
     }
-    for (int b = 0; b < B; b++)
+    for (int b = 0; b < B && poison != 3; b++)
         for (int i = 0; i < n[b]; i++)
             for (int h = 0; h < nh + nkv; h++) {
                 const int p = tot[b] - n[b] + i;
@@ -159,6 +165,10 @@ int main(int argc, char ** argv) {
                            f32 ? GSVK_TYPE_F32 : kv.type, (int64_t) nh * hd, lse, ws, wsb, nullptr)) {
         std::fprintf(stderr, "%s\n", gsvk::get_error());
         return 1;
+    }
+    if (poison == 3) {
+        std::printf("no access outside the buffers, workspace %zu\n", wsb);
+        return 0;
     }
     const auto got = [&](int64_t i) { return f32 ? (double) ((float *) out)[i] : dec(((uint16_t *) out)[i]); };
     double worst = 0, worst_l = 0;

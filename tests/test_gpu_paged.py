@@ -225,6 +225,102 @@ def test_long_sequences_split(gpu, lens, nh, nkv, hd):
     assert np.array_equal(a, b) and np.array_equal(la, lb)
 
 
+# Calls whose keys are divided among workgroups: a long chunk beside short ones, a single token, a draft,
+# nothing, and a chunk without old keys
+CUT = [(130, 5200), (1, 4000), (0, 0), (70, 900), (3, 2500), (33, 33), (0, 77)]
+
+
+@pytest.mark.parametrize("hd,nh,nkv,t", [(32, 3, 3, "f16"), (64, 4, 1, "bf16"), (128, 4, 2, "f16")])
+@pytest.mark.parametrize("kind", ["plain", "window", "prefix", "pages", "f32"])
+def test_chunks_cut_into_runs(gpu, hd, nh, nkv, t, kind):
+    bt = Batch(hd + len(kind), CUT, nh, nkv, hd, 32, t, tail=3)
+    if kind == "pages":
+        bt.table[0, ::9] = -1
+        bt.table[1, 3] = bt.n_pages
+        bt.table[3, :] = 2 ** 31 - 1
+    kv = bt.device(gpu)
+    assert gpu.attn_paged_workspace_bytes(kv, bt.tokens, nh, 130, 5200) > 0
+    a = _attn(gpu, bt, window=2222 if kind == "window" else 0,
+              prefix=[5150, 100, 3, 900, 0, 40, 5] if kind == "prefix" else None, out_t="f32" if kind == "f32" else None)
+    b = _attn(gpu, bt, window=2222 if kind == "window" else 0, check=False,
+              prefix=[5150, 100, 3, 900, 0, 40, 5] if kind == "prefix" else None, out_t="f32" if kind == "f32" else None)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_unseen_values_do_not_matter_when_cut(gpu):
+    """As test_unseen_values_do_not_matter, with the keys divided among workgroups."""
+    bt = Batch(17, CUT, 4, 2, 128, 32, "f16", stale=0.5)
+    want, wl = _attn(gpu, bt)
+    for b, (n, tot) in enumerate(bt.lens):
+        if n > 1:
+            bt.K[b][tot - 1], bt.V[b][tot - 1] = math.nan, math.nan
+    bt.kc[:], bt.vc[:] = math.nan, math.inf
+    bt.write()
+    got, gl = _attn(gpu, bt, check=False)
+    last = [int(bt.seq_start[b + 1]) - 1 for b, (n, _) in enumerate(bt.lens) if n > 1]
+    clean = [r for r in range(bt.T) if r not in last]
+    assert np.array_equal(got[clean], want[clean]) and np.array_equal(gl[clean], wl[clean])
+    assert all(np.isnan(got[r]).any() for r in last)
+
+
+@pytest.mark.parametrize("B", [300, 520])
+def test_many_sequences(gpu, B):
+    """More sequences than a workgroup has threads (and than the lists of equal runs hold), a long chunk
+    among them."""
+    lens = [(1 + (b % 3 == 0) * (b % 5), 1 + b % 70) for b in range(B)]
+    lens = [(n, max(n, t)) for n, t in lens]
+    lens[B // 2] = (150, 4000)
+    lens[B - 1] = (60, 1700)
+    lens[3] = (0, 5)
+    _attn(gpu, Batch(B, lens, 2, 1, 128, 16, "bf16", tail=1))
+
+
+def test_nothing_to_do(gpu):
+    """No rows, no sequences, sequences without rows: nothing is written and nothing fails."""
+    bt = Batch(18, [(0, 20), (0, 0)], 4, 2, 64, 16, "f16", tail=4)
+    _attn(gpu, bt)
+    kv = bt.device(gpu)
+    e = torch.empty((0, 4, 64), dtype=DT["f16"], device="cuda")
+    gpu.op_attn_paged(kv, e, 0.1, e, max_new=0)
+    gpu.op_paged_append(kv, e[:, :2], e[:, :2])
+    none = gpu.PagedKV(bt.dkc, bt.dvc, bt.dtable[:0], bt.dss[:1], bt.dlen[:0])
+    q = torch.full((4, 4, 64), 3.0, dtype=DT["f16"], device="cuda")
+    out = q.clone()
+    gpu.op_attn_paged(none, q, 0.1, out, max_new=4)
+    gpu.op_paged_append(none, q[:, :2], q[:, 2:])
+    torch.cuda.synchronize()
+    assert bool((out == 3.0).all()) and torch.equal(bt.dkc.cpu().nan_to_num(7.0), bt.kc.nan_to_num(7.0))
+
+
+def test_two_graphs_share_a_workspace(gpu):
+    """Two captured calls over one workspace, replayed in turn: nothing in it outlives a call."""
+    scale, sets = 0.125, []
+    bts = [Batch(71, CUT, 4, 1, 64, 32, "bf16"), Batch(72, [(1, 9000), (1, 30)], 4, 1, 64, 32, "bf16")]
+    need = [gpu.attn_paged_workspace_bytes(bt.device(gpu), bt.T, 4, max(bt.new), 9000) for bt in bts]
+    assert min(need) > 0
+    ws = torch.full((max(need),), 255, dtype=torch.uint8, device="cuda")
+    for bt in bts:
+        q, out = bt.q.cuda(), torch.zeros((bt.T, 4, 64), dtype=DT["bf16"], device="cuda")
+        call = lambda kv=bt.kv, q=q, out=out, bt=bt: gpu.op_attn_paged(kv, q, scale, out, max_new=max(bt.new), max_keys=9000, ws=ws)
+        call()
+        torch.cuda.synchronize()
+        want = out.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        sets.append((bt, out, want, g, q))       # (a graph reads the q that it was captured with)
+    for bt, out, want, _, _ in sets:
+        ref, _, dout, _ = bt.attn(scale)
+        assert np.all(np.abs(want.cpu().double().numpy() - ref) <= dout + rounding(np.abs(ref) + dout, "bf16"))
+    for _ in range(3):
+        for _, out, want, g, _ in sets:
+            out.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out, want, g, _ in sets:
+            assert torch.equal(out, want)
+
+
 def test_max_new_bounds_the_rows(gpu):
     """Rows past max_new are not computed and keep what they held."""
     bt = Batch(14, [(5, 40)], 2, 2, 32, 16, "f16")
