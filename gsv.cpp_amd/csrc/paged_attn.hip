@@ -80,7 +80,8 @@ struct PagedAttn {
     int nsplit;         // runs that a sequence of few rows is cut into
     int min_rows;       // of a chunk: sequences of fewer rows are few_tile's
     int chunk_groups;   // workgroups of chunks
-    int bal_most;       // row tiles of a head that there can be, if balanced
+    int bal_most;       // row tiles of a head that there can be (k_attn_paged_balanced)
+    int ordered;        // k_attn_paged_balanced: whole row tiles by length
     int few_rows;       // rows that a sequence of few rows can have
 };
 
@@ -851,10 +852,13 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
     chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds.chunk);
 }
 
-// Few row tiles of unequal length: the key tiles of all of them, in the order (head, sequence, row
-// tile, key), are cut into equal runs, one per workgroup (CUs that would wait for the longest row
-// tile share its keys). A row tile that a cut goes through is joined by k_attn_paged_join. Every workgroup computes
-// the same list of row tiles and running sums; the ids of an XCD take consecutive runs.
+// Row tiles of unequal length. Every workgroup computes the same list of row tiles and running sums of
+// their key tiles, then, by a.ordered,
+//   1  takes one whole row tile: the ids go from the longest to the shortest, so that the workgroups that share
+//      a CU, and those that come last, are not long ones by chance;
+//   0  takes a run of key tiles: those of all row tiles in the order (head, sequence, row tile, key) are
+//      cut into equal runs, one per workgroup, and the ids of an XCD take consecutive runs. A row tile that a
+//      cut goes through is joined by k_attn_paged_join. For few row tiles over many keys.
 constexpr int BAL_GROUPS = 512, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
 
 struct BalHead { int64_t run; int tiles, pad; };    // key tiles per workgroup, row tiles of a head
@@ -926,7 +930,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     __syncthreads();
     tiles = __builtin_amdgcn_readfirstlane(min(tiles, a.bal_most));   // (more only if seq_start does not ascend)
     if (tiles == 0) {
-        if (blockIdx.x == 0 && tid == 0) *a.bal_head = BalHead{1, 0, 0};
+        if (blockIdx.x == 0 && tid == 0 && !a.ordered) *a.bal_head = BalHead{1, 0, 0};
         return;
     }
     int units = 0;   // key tiles of a head
@@ -944,6 +948,28 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
     if (tid == 0) bal.units[tiles] = units;
     __syncthreads();
     units = __builtin_amdgcn_readfirstlane(units);
+    if (a.ordered) {
+        // heads fastest: an XCD keeps its heads
+        const int rank = (int) blockIdx.x / a.kv.n_kv, kvh = (int) blockIdx.x % a.kv.n_kv;
+        if (rank >= tiles) return;
+        for (int e = tid; e < tiles; e += CH_WAVES * 64) {
+            const int n = bal.units[e + 1] - bal.units[e];
+            int r = 0;
+            for (int i = 0; i < tiles; i++) {
+                const int x = bal.units[i + 1] - bal.units[i];
+                r += x > n || (x == n && i < e);
+            }
+            if (r == rank) bal.wave[0] = e;
+        }
+        __syncthreads();
+        const int e = __builtin_amdgcn_readfirstlane(bal.wave[0]);
+        const int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
+        const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
+        const Seq s = seq_of(a, b);
+        const Span sp = span_of(a, s, rt);
+        chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds.chunk);
+        return;
+    }
     const int64_t total = (int64_t) units * a.kv.n_kv;
     const int64_t share = (total + BAL_GROUPS - 1) / BAL_GROUPS;
     const int64_t run = max(share, (int64_t) min(BAL_LEAST, (units + tiles - 1) / tiles));
@@ -1092,7 +1118,7 @@ template <class T, int HD, int SL>
 __global__ void __launch_bounds__(256) k_attn_paged_join(PagedAttn a) {
     __shared__ MergeLds<HD, SL> lds;
     constexpr int X = CH_WAVES * (HD / 32), R = 256 / (HD / 8) / SL;
-    const int tiles = a.bal_most * a.kv.n_kv * X;
+    const int tiles = a.ordered ? 0 : a.bal_most * a.kv.n_kv * X;
     int i = blockIdx.x;
     if (i < tiles) {
         join_tile<T, HD>(a, i / X % a.bal_most, i / X / a.bal_most, i % X);
@@ -1110,23 +1136,32 @@ struct Plan {
     bool few, chunk;       // sequences of few rows can be there; chunks can
     int few_rows, few_qt, few_waves, few_tiles, few_split;
     int chunk_tiles;       // row tiles of the longest sequence
-    int balanced_tiles;    // 0: one row tile per workgroup; else the most row tiles that there can be per head
+    int deal;              // of chunks to workgroups (Deal)
+    int most_tiles;        // with lists: the most row tiles that there can be per head
 };
 
-// Whether equal runs of keys pay for their lists, second segments and joins. Estimated times in us: a
-// step of 64 keys takes `step` with one workgroup on a CU and up to twice that with two, so one row tile
-// per workgroup takes the longest row tile's steps or the chip's share of all, and runs the latter and
-// a fixed cost that grows with the partial results. `all` takes the other sequences of a batch as
-// 0.7 of the longest. Measured (one row tile per workgroup / runs): 2000 tokens of 32 heads of 128 over 8
-// 54 / 88, 2000 of 16 heads of 64 35 / 42, 4000 of 16 heads of 32 54 / 67; 2 x 256 tokens over 2900 keys,
-// 32 heads of 128 over 8 72 / 52, 64 tokens over 8000 keys 160 / 40, two chunks of 900 over 4900 keys beside
-// 22 single tokens 223 / 178, 4 x 512 tokens over 8100 keys 233 / 241.
-bool balanced_pays(int B, int hd, double tiles, int max_new, int64_t max_keys) {
+// How chunks are dealt to workgroups, by estimated times in us. A step of 64 keys takes `step` with one
+// workgroup on a CU and up to twice that with two. One row tile per workgroup takes the longest row tile's
+// steps or the chip's share of all; in the order of the grid two long ones can share a CU while the
+// chip holds about all of them (512 workgroups), by length they do not, at the price of the list. Equal
+// runs take the share and a fixed cost that grows with the partial results. `all` takes the other
+// sequences of a batch as 0.7 of the longest. Measured (us; grid order / by length / runs), heads of 128,
+// 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 233 / 224 / 246, two chunks of 700 to 1000 over 200 to
+// 4900 beside 22 single tokens 223 / 152 / 181, 3 prompts of 300 to 2500 70 / 77 / -, one of 2000 54 / 58 / 88,
+// 2 x 256 over 2900 72 / - / 52, 64 over 8000 160 / - / 40; heads of 64: 8 x 200 to 800 over up to 3800,
+// 16 over 8 - / 59 / 74, 6 x 100 to 700 over up to 3700, 32 over 8 of 128 127 / 102 / 131, a prompt of 2000, 16 over 16 35 / - / 42.
+enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
+Deal deal_of(int B, int hd, double tiles, int max_new, int64_t max_keys, bool lists) {
     const double step = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45, load = tiles / 256;
     const double longest = (double) max_keys / 64, mean = std::max(0.0, (double) max_keys - 0.5 * max_new) / 64;
-    const double slow = 1.1 * (1.0 + std::min(std::max(load - 1.0, 0.0), 1.0) * mean / std::max(longest, 1.0));
+    // (prompts from the start come by length in the grid's order too, once there are more than fit)
+    const double old = mean / std::max(longest, 1.0), shared = std::min({load - 1.0, 1.0, old > 0.7 ? 1.0 : 3.0 - load});
+    const double slow = 1.1 * (1.0 + std::max(shared, 0.0) * old);
     const double all = mean * tiles / 512 * 1.95 * step * (B > 1 ? 0.7 : 1.0);
-    return std::max(longest * slow * step, all) > all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
+    const double grid = std::max(longest * slow * step, all), length = B > 1 ? std::max(1.1 * longest * step, all) + 6 : 1e30;   // (one sequence's go well as they are)
+    const double runs = all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
+    if (!lists || grid <= std::min(length, runs)) return DEAL_GRID;
+    return length <= runs ? DEAL_LENGTH : DEAL_RUNS;
 }
 
 Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
@@ -1152,8 +1187,8 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
         p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);
         // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence
         const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS), most = tokens * group / CH_ROWS + B;
-        if (B <= BAL_SEQS && most <= BAL_TILES && balanced_pays(B, hd, (double) (least * n_kv), max_new, max_keys))
-            p.balanced_tiles = (int) most;
+        p.deal = deal_of(B, hd, (double) (least * n_kv), max_new, max_keys, B <= BAL_SEQS && most <= BAL_TILES);
+        if (p.deal != DEAL_GRID) p.most_tiles = (int) most;
     }
     return p;
 }
@@ -1163,8 +1198,8 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
 struct Space { size_t slots, few, ml, end; };
 Space space_of(const Plan & p, int64_t rows, int n_kv, int hd) {
     Space w{};
-    if (p.balanced_tiles) {
-        w.slots = (sizeof(BalHead) + (size_t) p.balanced_tiles * n_kv * sizeof(BalTile) + 255) / 256 * 256;
+    if (p.deal == DEAL_RUNS) {
+        w.slots = (sizeof(BalHead) + (size_t) p.most_tiles * n_kv * sizeof(BalTile) + 255) / 256 * 256;
         w.few = w.slots + 2 * (size_t) BAL_GROUPS * CH_ROWS * (size_t) (hd + 2) * sizeof(float);
     }
     w.ml = w.end = w.few;
@@ -1175,16 +1210,20 @@ Space space_of(const Plan & p, int64_t rows, int n_kv, int hd) {
     return w;
 }
 
+int64_t chunk_groups_of(const Plan & p, int B, int n_kv) {   // workgroups of chunks
+    if (!p.chunk) return 0;
+    return p.deal == DEAL_RUNS ? BAL_GROUPS : (int64_t) (p.deal == DEAL_LENGTH ? p.most_tiles : (int64_t) p.chunk_tiles * B) * n_kv;
+}
 int64_t groups_of(const Plan & p, int B, int n_kv) {   // workgroups of the first launch
     const int64_t few = (int64_t) p.few_tiles * p.few_split * n_kv * B;
-    return (p.chunk ? (p.balanced_tiles ? BAL_GROUPS : (int64_t) p.chunk_tiles * n_kv * B) : 0) + few;
+    return chunk_groups_of(p, B, n_kv) + few;
 }
 
 // rows of few rows that a workgroup of k_attn_paged_join takes, and its workgroups
 int join_rows(const Plan & p, int hd) { return 256 / (hd / 8) / (p.few_split > 4 ? 16 : 1); }
 int64_t join_groups_of(const Plan & p, int B, int n_kv, int hd) {
     const int64_t per = p.few_split > 1 ? (p.few_rows + join_rows(p, hd) - 1) / join_rows(p, hd) : 0;
-    return (int64_t) p.balanced_tiles * n_kv * (CH_WAVES * (hd / 32)) + per * n_kv * B;
+    return (p.deal == DEAL_RUNS ? (int64_t) p.most_tiles * n_kv * (CH_WAVES * (hd / 32)) : 0) + per * n_kv * B;
 }
 
 template <class T, int HD>
@@ -1200,10 +1239,11 @@ void launch_attn(PagedAttn a, const Plan & p, void * ws, hipStream_t st) {
     a.few_rows = p.few_rows;
     if (p.chunk) {
         a.min_rows = p.few ? FEW_ROWS + 1 : 1;
-        a.bal_most = p.balanced_tiles;
-        a.chunk_groups = p.balanced_tiles ? BAL_GROUPS : (int) ((int64_t) p.chunk_tiles * nkv * B);
+        a.bal_most = p.most_tiles;
+        a.ordered = p.deal == DEAL_LENGTH;
+        a.chunk_groups = (int) chunk_groups_of(p, a.kv.B, a.kv.n_kv);
         const dim3 grid((unsigned) groups_of(p, a.kv.B, a.kv.n_kv)), block(CH_WAVES * 64);
-        if (p.balanced_tiles) hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), grid, block, 0, st, a);
+        if (p.deal != DEAL_GRID) hipLaunchKernelGGL((k_attn_paged_balanced<T, HD>), grid, block, 0, st, a);
         else hipLaunchKernelGGL((k_attn_paged_chunk<T, HD>), grid, block, 0, st, a);
     } else {
         const dim3 grid((unsigned) (p.few_tiles * p.few_split), nkv, B), block((unsigned) p.few_waves * 64);
