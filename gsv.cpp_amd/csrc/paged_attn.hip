@@ -1182,6 +1182,8 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
         p.few_waves = !p.chunk && pairs * p.few_tiles <= 256 ? 8 : 4;
         const int64_t n = std::min((4096 + p.few_waves * pairs - 1) / (p.few_waves * pairs), max_keys / (256 * p.few_waves));
         p.few_split = (int) std::max<int64_t>(1, std::min<int64_t>(n, 64));
+        // (chunks of max_new tokens each, unless rows are padding: no launch to join what is hardly there)
+        if (p.chunk && tokens >= (int64_t) B * max_new) p.few_split = 1;
     }
     if (p.chunk) {
         p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);

@@ -427,6 +427,16 @@ class PagedKV:
                                 k.stride(0) if n_pages > 1 else 0, table.data_ptr(),
                                 table.stride(0) if B > 1 else cols, cols, B, seq_start.data_ptr(), kv_len.data_ptr())
         self._ref = C.byref(self.args)
+        self._ws = {}    # workspace bytes by the sizes of a call
+
+    def workspace_bytes(self, tokens, nh, max_new, max_keys, window=0):
+        key = (tokens, nh, max_new, max_keys, window)
+        n = self._ws.get(key)
+        if n is None:
+            if len(self._ws) > 4096:
+                self._ws.clear()
+            n = self._ws[key] = int(lib().gsvk_attn_paged_workspace_bytes(self._ref, *key))
+        return n
 
 
 def _paged_stream(kv, stream, what):
@@ -444,8 +454,11 @@ _torch_cuda = None   # torch's current device, and the handle of its current str
 def _load_torch():
     global _torch_cuda
     import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the stream object costs 3 us more)
-    _torch_cuda = (torch.cuda.current_device, raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
+    torch.cuda.current_device()   # (initialises)
+    # (the public forms cost 3 us more: a stream object, a check of the initialisation)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _torch_cuda = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
+                   raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
 
 
 def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=False, pos=None, n_bad=None,
@@ -482,7 +495,7 @@ def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=Fals
 
 
 def attn_paged_workspace_bytes(kv, tokens, nh, max_new, max_keys, window=0) -> int:
-    return int(lib().gsvk_attn_paged_workspace_bytes(kv._ref, tokens, nh, max_new, max_keys, window))
+    return kv.workspace_bytes(tokens, nh, max_new, max_keys, window)
 
 
 def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0, prefix=None, ws=None, stream=None):
@@ -505,7 +518,7 @@ def op_attn_paged(kv, q, scale, out, max_new, max_keys=None, lse=None, window=0,
     if ws is None:
         if stream is not None and stream != _torch_cuda[1](dev):
             raise ValueError("attn_paged: a stream other than torch's current one needs a ws of its own")
-        wn = lib().gsvk_attn_paged_workspace_bytes(kv._ref, T, nh, max_new, max_keys, window)
+        wn = kv.workspace_bytes(T, nh, max_new, max_keys, window)
         if wn:
             import torch
             ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
