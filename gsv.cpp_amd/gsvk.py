@@ -353,19 +353,29 @@ def op_qkv_attn(wq, wd, bias, res, r, ln_bias, wb, k, v, kv_begin, col, scale, o
              _p(kv_begin), _p(col), scale, _p(out), _p(oq), _p(od), _p(ln_out), _stream(stream)), "qkv_attn")
 
 
+_TYPES = {}          # torch dtype -> GGML type number, filled by _load_torch
+_torch_cuda = None   # torch's current device, and the handle of its current stream on a device
+_torch_types = None  # torch.int32, torch.float32
+
+
+def _load_torch():
+    global _torch_cuda, _torch_types
+    import torch
+    torch.cuda.current_device()   # (initialises)
+    _TYPES.update({torch.float32: GSVK_TYPE_F32, torch.float16: GSVK_TYPE_F16, torch.bfloat16: GSVK_TYPE_BF16})
+    _torch_types = (torch.int32, torch.float32)
+    # (the public forms cost 3 us more: a stream object, a check of the initialisation)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _torch_cuda = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
+                   raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
+
+
 def _gsvk_type(dtype):
     """GGML type number of a torch dtype (F32, F16 or BF16)."""
     t = _TYPES.get(dtype)
     if t is None:
-        import torch
-        _TYPES.update({torch.float32: GSVK_TYPE_F32, torch.float16: GSVK_TYPE_F16, torch.bfloat16: GSVK_TYPE_BF16})
-        t = _TYPES.get(dtype)
-        if t is None:
-            raise ValueError(f"gsvk: {dtype} is not a type of the paged-cache operators")
+        raise ValueError(f"gsvk: {dtype} is not a type of the paged-cache operators")
     return t
-
-
-_TYPES = {}
 
 
 def _rows_of(t, what, width, device):
@@ -390,13 +400,11 @@ def _int32(t, what, shape, device):
 
 
 def _int32_ok(t, shape, device):
-    return t.element_size() == 4 and not t.is_floating_point() and not t.is_complex() and t.shape == shape \
-        and t.is_contiguous() and t.get_device() == device
+    return t.dtype is _torch_types[0] and t.shape == shape and t.is_contiguous() and t.get_device() == device
 
 
 def _f32_ok(t, shape, device):
-    return t.element_size() == 4 and t.is_floating_point() and t.shape == shape and t.is_contiguous() \
-        and t.get_device() == device
+    return t.dtype is _torch_types[1] and t.shape == shape and t.is_contiguous() and t.get_device() == device
 
 
 class PagedKV:
@@ -406,6 +414,7 @@ class PagedKV:
     operators read the tensors' contents when they run."""
 
     def __init__(self, k, v, table, seq_start, kv_len):
+        _load_torch()
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
             raise ValueError("PagedKV: k and v must be [n_pages][n_kv][page_size][hd] alike")
         n_pages, n_kv, page, hd = k.shape
@@ -415,7 +424,7 @@ class PagedKV:
         dev = k.get_device()
         if not k.is_cuda or any(t.get_device() != dev for t in (v, table, seq_start, kv_len)):
             raise ValueError("PagedKV: every tensor must be on the cache's device")
-        if table.dim() != 2 or str(table.dtype) != "torch.int32" or (table.shape[1] != 1 and table.stride(1) != 1):
+        if table.dim() != 2 or table.dtype is not _torch_types[0] or (table.shape[1] != 1 and table.stride(1) != 1):
             raise ValueError("PagedKV: table must be [B][cols] int32 with contiguous rows")
         B, cols = table.shape
         _int32(seq_start, "PagedKV: seq_start", (B + 1,), dev)
@@ -441,24 +450,9 @@ class PagedKV:
 
 def _paged_stream(kv, stream, what):
     """The stream of a call (torch's current one by default), on the cache's device."""
-    if _torch_cuda is None:
-        _load_torch()
     if _torch_cuda[0]() != kv.device:
         raise ValueError(f"{what}: the cache is on device {kv.device}, which is not the current one")
     return _torch_cuda[1](kv.device) if stream is None else stream
-
-
-_torch_cuda = None   # torch's current device, and the handle of its current stream on a device
-
-
-def _load_torch():
-    global _torch_cuda
-    import torch
-    torch.cuda.current_device()   # (initialises)
-    # (the public forms cost 3 us more: a stream object, a check of the initialisation)
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    _torch_cuda = (getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device,
-                   raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
 
 
 def op_paged_append(kv, k, v, q=None, q_out=None, cos=None, sin=None, pairs=False, pos=None, n_bad=None,

@@ -582,7 +582,8 @@ int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, const void * 
  * (infinities and NaN too).
  * max_new: the most new tokens of any sequence (rows past it are not computed); max_keys: the most
  * keys of any sequence, which only decides how the work is split. scale > 0; tokens * nh < 2^31.
- * ws: gsvk_attn_paged_workspace_bytes() bytes of device memory of the same arguments (NULL if 0);
+ * out and lse must not overlap q. ws: gsvk_attn_paged_workspace_bytes() bytes of device memory of the
+ * same arguments (NULL if 0), 16-byte aligned;
  * nothing in it outlives the call. Results do not depend on what else runs, and are the same bits
  * for the same arguments. */
 size_t gsvk_attn_paged_workspace_bytes(const gsvk_paged_kv * kv, int64_t tokens, int nh, int max_new,

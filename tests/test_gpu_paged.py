@@ -263,6 +263,25 @@ def test_unseen_values_do_not_matter_when_cut(gpu):
     assert all(np.isnan(got[r]).any() for r in last)
 
 
+def test_unequal_chunks(gpu):
+    """Enough row tiles of unequal length for the launch to take them by length: long chunks over old
+    keys, a single token and a draft beside them."""
+    bt = Batch(19, [(700, 2600), (1, 1900), (540, 1500), (380, 900), (5, 40), (0, 9)], 32, 8, 32, 16, "f16", tail=1)
+    bt.table[2, 11] = -1
+    _attn(gpu, bt)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("form", ["steps", "chunk"])
+def test_small_values(gpu, form, t):
+    """Keys and values below the type's normal range (fp16 subnormals), queries large: nothing is flushed."""
+    bt = Batch(20, FORMS[form], 4, 2, 64, 16, t, v_scale=2.0 ** -17, q_scale=2.0 ** 9)
+    for b in range(bt.B):
+        bt.K[b] = (bt.K[b].float() * 2.0 ** -16).to(DT[t])
+    bt.write()
+    _attn(gpu, bt, scale=2.0 ** 7)
+
+
 @pytest.mark.parametrize("B", [300, 520])
 def test_many_sequences(gpu, B):
     """More sequences than a workgroup has threads (and than the lists of equal runs hold), a long chunk
