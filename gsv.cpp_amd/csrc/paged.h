@@ -38,6 +38,10 @@ __device__ __forceinline__ void pg_unpack8(const uint4 & u, float (&x)[8]) {
 
 constexpr int PG_MAX_KEYS = 1 << 26;   // of a sequence (sums of key tiles over a call stay in 31 bits)
 
+// Batch arrays, which no store of a kernel reaches: read as constants, so that a uniform index gives
+// scalar loads wherever they stand.
+typedef const __attribute__((address_space(4))) int32_t pg_const;
+
 // gsvk_paged_kv as the kernels take it. Everything that comes from device memory is checked where
 // it is read: row ranges are cut to [0, tokens), page numbers to the cache.
 struct PagedView {
@@ -57,12 +61,12 @@ struct PagedView {
 
     // the new rows of sequence b
     __device__ __forceinline__ int64_t row0(int b) const {
-        const int64_t s = seq_start[b];
+        const int64_t s = ((pg_const *) seq_start)[b];
         return s < 0 ? 0 : s > tokens ? tokens : s;
     }
     // keys of sequence b that the table has room for
     __device__ __forceinline__ int keys(int b) const {
-        int64_t n = kv_len[b];
+        int64_t n = ((pg_const *) kv_len)[b];
         const int64_t cap = (int64_t) table_cols << page_shift;
         n = n < 0 ? 0 : n > cap ? cap : n;
         return n > PG_MAX_KEYS ? PG_MAX_KEYS : (int) n;

@@ -48,7 +48,6 @@ typedef float pg_f16 __attribute__((ext_vector_type(16)));
 typedef short pg_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) pg_s4 pg_lds4;
 typedef __attribute__((address_space(3))) uint16_t pg_lds1;
-typedef const __attribute__((address_space(4))) int32_t pg_table;   // (no store of these kernels reaches it: scalar loads)
 
 constexpr int FEW_ROWS = 32;          // rows of a sequence up to which k_attn_paged_few takes it
 constexpr int FEW_KEYS = 32;
@@ -165,10 +164,10 @@ __device__ __forceinline__ Seq seq_of(const PagedAttn & a, int b) {
     s.row0 = a.kv.row0(b);
     const int64_t n = a.kv.row0(b + 1) - s.row0;
     s.keys = a.kv.keys(b);
-    s.p0 = (int64_t) a.kv.kv_len[b] - n;
+    s.p0 = (int64_t) ((pg_const *) a.kv.kv_len)[b] - n;
     s.n = n < 0 ? 0 : n > a.max_new ? a.max_new : (int) n;
     s.rows = s.n * a.group;
-    s.prefix = a.prefix ? a.prefix[b] : 0;
+    s.prefix = a.prefix ? ((pg_const *) a.prefix)[b] : 0;
     return s;
 }
 __device__ __forceinline__ int key_lo(const PagedAttn & a, const Seq & s, int tok) {
@@ -182,7 +181,7 @@ __device__ __forceinline__ int key_hi(const Seq & s, int tok) {
 }
 
 // Page of a key (uniform over the wave), -1 if it has none
-__device__ __forceinline__ int page_of(const PagedAttn & a, pg_table * tb, int key) {
+__device__ __forceinline__ int page_of(const PagedAttn & a, pg_const * tb, int key) {
     const int col = key >> a.kv.page_shift;
     const int pg = col < a.kv.table_cols ? tb[col] : -1;
     return pg >= 0 && pg < a.kv.n_pages ? pg : -1;
@@ -266,7 +265,7 @@ __device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, in
     const int per = (nblk + a.nsplit - 1) / a.nsplit;
     const int blk0 = blk_a + min(nblk, split * per), blk1 = blk_a + min(nblk, (split + 1) * per);
 
-    pg_table * tb = (pg_table *) (a.kv.table + b * a.kv.table_stride);
+    pg_const * tb = (pg_const *) (a.kv.table + b * a.kv.table_stride);
     uint16_t * sv = reinterpret_cast<uint16_t *>(s_mem + wave * VB);
     uint4 kr[2][NK], vr[NV];
     int pg[2];
@@ -546,7 +545,7 @@ __device__ __forceinline__ void chunk_tile(const PagedAttn & a, const Seq & s, i
 #pragma unroll
         for (int c = 0; c < NK; c++) qf[c] = v8_of<T>(*reinterpret_cast<const uint4 *>(qp + 16 * c));
     }
-    pg_table * tb = (pg_table *) (a.kv.table + b * a.kv.table_stride);
+    pg_const * tb = (pg_const *) (a.kv.table + b * a.kv.table_stride);
 
     // A wave's loads of a tile: load j brings the 64 16-byte pieces from piece (j CH_WAVES + wave) * 64 on,
     // all within one group of 16 keys, so within one page.
