@@ -562,7 +562,7 @@ typedef struct gsvk_rope {
  * itself where both are dense and of one type; q and q_out NULL (nh 0): keys and values only.
  * A row whose key has no page, a negative index or a position outside [0, rope->rows) is not
  * written (q_out neither) and counted in *n_bad (device int32, added to; may be NULL). Two rows of
- * one call must not name the same slot. k_out, v_out of other slots keep what they held.
+ * one call must not name the same slot. Other slots keep what they held.
  * Stands for the append of src/gsv_ar.cpp:398-399, there into a dense cache without rotation. */
 int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, const void * k, const void * v, int x_type,
                          int64_t tokens, int nh, int64_t q_stride, int64_t k_stride, int64_t v_stride,
