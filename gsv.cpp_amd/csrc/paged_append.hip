@@ -154,9 +154,10 @@ extern "C" int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, co
     GSVK_TRY(paged_view(kv, tokens, "paged_append", view));
     GSVK_REQUIRE(x_type == GSVK_TYPE_F32 || x_type == kv->type,
                  "paged_append: x_type %d is neither F32 nor the cache's type", x_type);
-    GSVK_REQUIRE((nh > 0) == (q != nullptr) && (q != nullptr) == (q_out != nullptr) && nh >= 0 && nh <= 65535,
-                 "paged_append: q, q_out and nh (at most 65535) go together");
-    if (tokens == 0 || kv->B == 0) return GSVK_OK;
+    GSVK_REQUIRE(nh >= 0 && nh <= 65535, "paged_append: nh %d out of range", nh);
+    if (tokens == 0 || kv->B == 0) return GSVK_OK;   // (an empty array may be NULL)
+    GSVK_REQUIRE((nh > 0) == (q != nullptr) && (q != nullptr) == (q_out != nullptr),
+                 "paged_append: q, q_out and nh go together");
     GSVK_REQUIRE(k && v, "paged_append: k and v must be given");
     const int64_t es = x_type == GSVK_TYPE_F32 ? 4 : 2;
     GSVK_REQUIRE((!q || q_stride >= (int64_t) nh * kv->hd || tokens == 1)

@@ -78,6 +78,12 @@ def test_nothing_to_do_is_no_error():
     assert _attn(_kv(), tokens=0) == 0 and _attn(_kv(B=0)) == 0 and _attn(_kv(), max_new=0) == 0
 
 
+def test_empty_arrays_may_be_null():
+    """An empty tensor has no address: a step without rows passes through."""
+    assert _append(_kv(), tokens=0, q=None, k=None, v=None, q_out=None) == 0
+    assert _attn(_kv(), tokens=0, q=None, out=None) == 0
+
+
 def _ws(kv, tokens, nh, max_new, max_keys):
     return gsvk.lib().gsvk_attn_paged_workspace_bytes(C.byref(kv), tokens, nh, max_new, max_keys, 0)
 
