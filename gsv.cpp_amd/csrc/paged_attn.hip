@@ -18,9 +18,10 @@
 //                       belongs to the wave, so the loop has no barrier. Bound by HBM.
 //   k_attn_paged_chunk  longer chunks: 4 waves of 32 rows share key tiles of 64 in LDS (double
 //                       buffered), v_mfma_f32_32x32x16.
-// Where that makes too few workgroups, or too unequal ones, keys are divided too: k_attn_paged_few cuts
-// each row tile into nsplit runs of keys, k_attn_paged_balanced all row tiles together into equal
-// runs; (maximum, sum, unnormalised output) of the parts are joined by k_attn_paged_join.
+// Where that makes too few workgroups keys are divided too: k_attn_paged_few cuts each row tile into
+// nsplit runs of keys, k_attn_paged_balanced all row tiles together into equal runs; (maximum, sum,
+// unnormalised output) of the parts are joined by k_attn_paged_join. Where there are enough, but unequal
+// ones, k_attn_paged_balanced starts them from the longest to the shortest.
 //
 // Softmax. Exponents are base 2. The reference exponent m of a row is not its running maximum but
 // follows it: it is moved (and O, l rescaled) only when a score exceeds it by more than 2^12, to
@@ -193,7 +194,7 @@ __device__ __forceinline__ int64_t key_at(const PagedAttn & a, int pg, int kvh, 
            + (((int64_t) kvh << a.kv.page_shift) + (key & ((1 << a.kv.page_shift) - 1))) * HD;
 }
 
-// Store 8 output values of a row: final, or a split's unnormalised ones
+// Store 8 output values of a row
 template <class T>
 __device__ __forceinline__ void store8(const PagedAttn & a, int64_t row, int col, const float (&x)[8]) {
     const int64_t at = row * a.out_stride + col;
@@ -228,11 +229,11 @@ struct FewLds {
     float ml[NW][QT * 16][2];
 };
 
-// QT tiles of 16 rows of (head kvh, sequence b) from row tile rt on, keys of one of nsplit runs, by a
-// workgroup of NW waves
+// QT tiles of 16 rows (row tile rt) of (head kvh, sequence b), keys of one of nsplit runs, by a workgroup
+// of NW waves; sequences of more than FEW_ROWS rows are chunks
 template <class T, int HD, int QT, int NW>
-__device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, int rt, int split, int min_rows,
-                                         int max_rows, FewLds<HD, QT, NW> & lds) {
+__device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, int rt, int split,
+                                         FewLds<HD, QT, NW> & lds) {
     constexpr int C = HD / 8, NV = FEW_KEYS * C / 64, NK = HD / 32, DT = HD / 16, OS = HD + 4;
     constexpr int VB = few_wave_lds<HD>();
     char * s_mem = lds.mem;
@@ -242,7 +243,7 @@ __device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, in
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Seq s = seq_of(a, b);
     const int r0 = rt * QT * 16;
-    if (r0 >= s.rows || s.rows < min_rows || s.rows > max_rows) return;
+    if (r0 >= s.rows || s.rows > FEW_ROWS) return;
     const int nh = a.group * a.kv.n_kv;
     const int tok0 = r0 / a.group, tok1 = min(r0 + QT * 16, s.rows) - 1, tokl = tok1 / a.group;
     const int klo = key_lo(a, s, tok0), khi = key_hi(s, tokl);
@@ -461,7 +462,7 @@ __device__ __forceinline__ void few_tile(const PagedAttn & a, int b, int kvh, in
 template <class T, int HD, int QT, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) k_attn_paged_few(PagedAttn a) {
     __shared__ __align__(16) FewLds<HD, QT, NW> lds;
-    few_tile<T, HD, QT, NW>(a, blockIdx.z, blockIdx.y, blockIdx.x / a.nsplit, blockIdx.x % a.nsplit, 1, FEW_ROWS, lds);
+    few_tile<T, HD, QT, NW>(a, blockIdx.z, blockIdx.y, blockIdx.x / a.nsplit, blockIdx.x % a.nsplit, lds);
 }
 
 // ---- chunks ----------------------------------------------------------------------------------------
@@ -827,7 +828,7 @@ union MixLds {
 template <class T, int HD>
 __device__ __forceinline__ void few_beside(const PagedAttn & a, MixLds<HD> & lds) {
     const int f = (int) blockIdx.x - a.chunk_groups, split = f % a.nsplit, kvh = f / a.nsplit % a.kv.n_kv;
-    few_tile<T, HD, 2, CH_WAVES>(a, f / a.nsplit / a.kv.n_kv, kvh, 0, split, 1, FEW_ROWS, lds.few);
+    few_tile<T, HD, 2, CH_WAVES>(a, f / a.nsplit / a.kv.n_kv, kvh, 0, split, lds.few);
 }
 
 // One row tile per workgroup, all its keys. (head, sequence) fastest, then the row tiles from each
@@ -858,7 +859,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
 //   0  takes a run of key tiles: those of all row tiles in the order (head, sequence, row tile, key) are
 //      cut into equal runs, one per workgroup, and the ids of an XCD take consecutive runs. A row tile that a
 //      cut goes through is joined by k_attn_paged_join. For few row tiles over many keys.
-constexpr int BAL_GROUPS = 512, BAL_SEQS = 512, BAL_TILES = 1024, BAL_LEAST = 4;
+constexpr int BAL_GROUPS = 512, BAL_SEQS = 4096, BAL_TILES = 1536, BAL_LEAST = 4, BAL_SORT = 256;
 
 struct BalHead { int64_t run; int tiles, pad; };    // key tiles per workgroup, row tiles of a head
 struct BalTile { int first, num, b, rt; };          // a row tile's place in its head's list of key tiles
@@ -866,7 +867,7 @@ template <int HD>
 constexpr size_t bal_slot() { return (size_t) CH_ROWS * (HD + 2); }   // floats
 
 struct BalLds {
-    int tiles[BAL_SEQS + 1];    // row tiles before each sequence
+    uint16_t tiles[BAL_SEQS + 1];   // row tiles before each sequence (two workgroups fit a CU's LDS with heads of 128)
     int units[BAL_TILES + 1];   // key tiles before each row tile of a head
     int wave[CH_WAVES];
 };
@@ -893,7 +894,8 @@ __device__ __forceinline__ int scan_group(int x, int * s_wave, int & total) {
     return before + y - x;
 }
 // the last i in [0, n) with p[i] <= x (p ascending, p[0] <= x)
-__device__ __forceinline__ int last_le(const int * p, int n, int x) {
+template <typename I>
+__device__ __forceinline__ int last_le(const I * p, int n, int x) {
     int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -922,10 +924,10 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
             if (s.rows >= a.min_rows) n = min((s.rows + CH_ROWS - 1) / CH_ROWS, a.bal_most);
         }
         n = scan_group(n, bal.wave, add);
-        if (b < a.kv.B) bal.tiles[b] = tiles + n;
-        tiles += add;
+        if (b < a.kv.B) bal.tiles[b] = (uint16_t) min(tiles + n, 0xffff);
+        tiles = min(tiles + add, 0xffff);
     }
-    if (tid == 0) bal.tiles[a.kv.B] = tiles;
+    if (tid == 0) bal.tiles[a.kv.B] = (uint16_t) tiles;
     __syncthreads();
     tiles = __builtin_amdgcn_readfirstlane(min(tiles, a.bal_most));   // (more only if seq_start does not ascend)
     if (tiles == 0) {
@@ -951,19 +953,22 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         // heads fastest: an XCD keeps its heads
         const int rank = (int) blockIdx.x / a.kv.n_kv, kvh = (int) blockIdx.x % a.kv.n_kv;
         if (rank >= tiles) return;
-        for (int e = tid; e < tiles; e += CH_WAVES * 64) {
-            const int n = bal.units[e + 1] - bal.units[e];
-            int r = 0;
-            for (int i = 0; i < tiles; i++) {
-                const int x = bal.units[i + 1] - bal.units[i];
-                r += x > n || (x == n && i < e);
+        int e = rank;
+        if (tiles <= BAL_SORT) {   // (the count is quadratic, and of more every CU gets several)
+            if (tid < tiles) {
+                const int n = bal.units[tid + 1] - bal.units[tid];
+                int r = 0;
+                for (int i = 0; i < tiles; i++) {
+                    const int x = bal.units[i + 1] - bal.units[i];
+                    r += x > n || (x == n && i < tid);
+                }
+                if (r == rank) bal.wave[0] = tid;
             }
-            if (r == rank) bal.wave[0] = e;
+            __syncthreads();
+            e = __builtin_amdgcn_readfirstlane(bal.wave[0]);
         }
-        __syncthreads();
-        const int e = __builtin_amdgcn_readfirstlane(bal.wave[0]);
         const int b = __builtin_amdgcn_readfirstlane(last_le(bal.tiles, a.kv.B, e));
-        const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
+        const int rt = e - __builtin_amdgcn_readfirstlane((int) bal.tiles[b]);
         const Seq s = seq_of(a, b);
         const Span sp = span_of(a, s, rt);
         chunk_tile<T, HD>(a, s, b, kvh, rt, sp.first, sp.first + sp.num, nullptr, lds.chunk);
@@ -989,7 +994,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         const int first = __builtin_amdgcn_readfirstlane(bal.units[e]);
         const int num = __builtin_amdgcn_readfirstlane(bal.units[e + 1]) - first;
         const int t1 = (int) min((int64_t) num, t0 + left);
-        const int rt = e - __builtin_amdgcn_readfirstlane(bal.tiles[b]);
+        const int rt = e - __builtin_amdgcn_readfirstlane((int) bal.tiles[b]);
         const Span sp = span_of(a, s, rt);
         float * part = nullptr;
         if (t1 - t0 < num) part = a.bal_part + (int64_t) (2 * w + more) * bal_slot<HD>();
@@ -1150,14 +1155,17 @@ struct Plan {
 // 2 x 256 over 2900 72 / - / 52, 64 over 8000 160 / - / 40; heads of 64: 8 x 200 to 800 over up to 3800,
 // 16 over 8 - / 59 / 74, 6 x 100 to 700 over up to 3700, 32 over 8 of 128 127 / 102 / 131, a prompt of 2000, 16 over 16 35 / - / 42.
 enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
-Deal deal_of(int B, int hd, double tiles, int max_new, int64_t max_keys, bool lists) {
+Deal deal_of(int B, int hd, double tiles, double groups, int max_new, int64_t max_keys, bool lists) {
     const double step = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45, load = tiles / 256;
     const double longest = (double) max_keys / 64, mean = std::max(0.0, (double) max_keys - 0.5 * max_new) / 64;
     // (prompts from the start come by length in the grid's order too, once there are more than fit)
     const double old = mean / std::max(longest, 1.0), shared = std::min({load - 1.0, 1.0, old > 0.7 ? 1.0 : 3.0 - load});
     const double slow = 1.1 * (1.0 + std::max(shared, 0.0) * old);
     const double all = mean * tiles / 512 * 1.95 * step * (B > 1 ? 0.7 : 1.0);
-    const double grid = std::max(longest * slow * step, all), length = B > 1 ? std::max(1.1 * longest * step, all) + 6 : 1e30;   // (one sequence's go well as they are)
+    // (a workgroup of the grid beyond a sequence's rows costs its start: a chunk of 4096 tokens beside 255 single
+    // ones, 32 over 8 of 128, 937 us of which 0.6 ms are such workgroups; from the list 361)
+    const double grid = std::max(longest * slow * step, all) + (groups - tiles) / 512;
+    const double length = B > 1 ? std::max(1.1 * longest * step, all) + 6 + B / 512.0 : 1e30;   // (one sequence's go well as they are)
     const double runs = all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
     if (!lists || grid <= std::min(length, runs)) return DEAL_GRID;
     return length <= runs ? DEAL_LENGTH : DEAL_RUNS;
@@ -1186,9 +1194,11 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
     }
     if (p.chunk) {
         p.chunk_tiles = (int) ((rows + CH_ROWS - 1) / CH_ROWS);
-        // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence
-        const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS), most = tokens * group / CH_ROWS + B;
-        p.deal = deal_of(B, hd, (double) (least * n_kv), max_new, max_keys, B <= BAL_SEQS && most <= BAL_TILES);
+        // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence that has more than few
+        const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS);
+        const int64_t most = tokens * group / CH_ROWS + (p.few ? std::min<int64_t>(B, tokens * group / (FEW_ROWS + 1)) : B);
+        p.deal = deal_of(B, hd, (double) (least * n_kv), (double) p.chunk_tiles * n_kv * B, max_new, max_keys,
+                         B <= BAL_SEQS && most <= BAL_TILES);
         if (p.deal != DEAL_GRID) p.most_tiles = (int) most;
     }
     return p;

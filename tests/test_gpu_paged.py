@@ -294,6 +294,17 @@ def test_many_sequences(gpu, B):
     _attn(gpu, Batch(B, lens, 2, 1, 128, 16, "bf16", tail=1))
 
 
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("chunks", [1, 3])
+def test_chunks_among_many_sequences(gpu, chunks, window):
+    """Prompts beside so many single tokens that whole row tiles are taken from a list (a grid of every sequence's
+    row tiles would be empty but for a few): in the order of their lengths, and as they come where they are many."""
+    lens = [(1, 1 + b % 90) for b in range(256)]
+    for i in range(chunks):
+        lens[100 * i + 7] = (1500 - i, 1500)
+    _attn(gpu, Batch(21, lens, 8, 1, 32, 16, "f16", tail=1), window=window)
+
+
 def test_nothing_to_do(gpu):
     """No rows, no sequences, sequences without rows: nothing is written and nothing fails."""
     bt = Batch(18, [(0, 20), (0, 0)], 4, 2, 64, 16, "f16", tail=4)
@@ -302,6 +313,7 @@ def test_nothing_to_do(gpu):
     e = torch.empty((0, 4, 64), dtype=DT["f16"], device="cuda")
     gpu.op_attn_paged(kv, e, 0.1, e, max_new=0)
     gpu.op_paged_append(kv, e[:, :2], e[:, :2])
+    gpu.op_paged_append(kv, e[:, :2], e[:, :2], q=e, q_out=e.clone())
     none = gpu.PagedKV(bt.dkc, bt.dvc, bt.dtable[:0], bt.dss[:1], bt.dlen[:0])
     q = torch.full((4, 4, 64), 3.0, dtype=DT["f16"], device="cuda")
     out = q.clone()

@@ -68,3 +68,11 @@ def test_malformed_batches_stay_in_bounds(check, args):
     """seq_start that descends, overlaps and leaves the rows, kv_len of any value: nothing outside the
     buffers is touched (what the rows get is not defined)."""
     _run(check, args)
+
+
+@pytest.mark.parametrize("poison", [0, 3])
+def test_chunks_among_many_sequences_in_bounds(check, poison):
+    """More row tiles of chunks, taken whole from the list, than are put in order; as they should be (0) and with
+    a malformed batch (3)."""
+    lens = "1500:1500 1500:1500 " + "1:9 " * 120 + "1500:1500 " + "1:40 " * 132
+    _run(check, f"32 0 8 1 16 16 0 0 {poison} 1 {lens}")
