@@ -1034,15 +1034,25 @@ __device__ __forceinline__ void join_tile(const PagedAttn & a, int e, int kvh, i
     if (r >= s.rows) return;
     const bool late = w0 * hd.run < u0;   // the first part is not its workgroup's first
     float M = M_NONE, L = 0.0f, x[4] = {};
-    for (int w = w0; w <= w1; w++) {
-        const float * part = a.bal_part + (2 * (int64_t) w + (w == w0 && late)) * bal_slot<HD>();
-        const float2 ml = *reinterpret_cast<const float2 *>(part + CH_ROWS * HD + 2 * rl);
-        const float4 u = *reinterpret_cast<const float4 *>(part + ((x0 * 4 + vq) * 64 + lane) * 4);
-        const float mn = fmaxf(M, ml.x), c = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml.x - mn);
-        M = mn;
-        L = __builtin_fmaf(L, c, ml.y * f);
-        x[0] = __builtin_fmaf(x[0], c, u.x * f); x[1] = __builtin_fmaf(x[1], c, u.y * f);
-        x[2] = __builtin_fmaf(x[2], c, u.z * f); x[3] = __builtin_fmaf(x[3], c, u.w * f);
+    for (int w = w0; w <= w1; w += 4) {   // (four parts' loads in flight)
+        float2 ml[4];
+        float4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int wi = min(w + i, w1);
+            const float * part = a.bal_part + (2 * (int64_t) wi + (wi == w0 && late)) * bal_slot<HD>();
+            ml[i] = *reinterpret_cast<const float2 *>(part + CH_ROWS * HD + 2 * rl);
+            u[i] = *reinterpret_cast<const float4 *>(part + ((x0 * 4 + vq) * 64 + lane) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (w + i > w1) break;
+            const float mn = fmaxf(M, ml[i].x), c = __builtin_amdgcn_exp2f(M - mn), f = __builtin_amdgcn_exp2f(ml[i].x - mn);
+            M = mn;
+            L = __builtin_fmaf(L, c, ml[i].y * f);
+            x[0] = __builtin_fmaf(x[0], c, u[i].x * f); x[1] = __builtin_fmaf(x[1], c, u[i].y * f);
+            x[2] = __builtin_fmaf(x[2], c, u[i].z * f); x[3] = __builtin_fmaf(x[3], c, u[i].w * f);
+        }
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
@@ -1155,9 +1165,9 @@ struct Plan {
 // 2 x 256 over 2900 72 / - / 52, 64 over 8000 160 / - / 40; heads of 64: 8 x 200 to 800 over up to 3800,
 // 16 over 8 - / 59 / 74, 6 x 100 to 700 over up to 3700, 32 over 8 of 128 127 / 102 / 131, a prompt of 2000, 16 over 16 35 / - / 42.
 enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
-Deal deal_of(int B, int hd, double tiles, double groups, int max_new, int64_t max_keys, bool lists) {
+Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mean_keys, bool lists) {
     const double step = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45, load = tiles / 256;
-    const double longest = (double) max_keys / 64, mean = std::max(0.0, (double) max_keys - 0.5 * max_new) / 64;
+    const double longest = keys / 64, mean = mean_keys / 64;
     // (prompts from the start come by length in the grid's order too, once there are more than fit)
     const double old = mean / std::max(longest, 1.0), shared = std::min({load - 1.0, 1.0, old > 0.7 ? 1.0 : 3.0 - load});
     const double slow = 1.1 * (1.0 + std::max(shared, 0.0) * old);
@@ -1174,20 +1184,31 @@ Deal deal_of(int B, int hd, double tiles, double groups, int max_new, int64_t ma
 Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, int64_t max_keys, int window) {
     Plan p{};
     if (max_new > tokens) max_new = (int) tokens;
-    if (window && max_keys > (int64_t) window + max_new) max_keys = (int64_t) window + max_new;   // (a row tile's)
+    max_keys = std::min<int64_t>(max_keys, PG_MAX_KEYS);
+    // the most keys of a row tile (of `some` rows): a window's and its own tokens'
+    const auto seen = [&](int64_t some) {
+        return window ? std::min(max_keys, window + std::min<int64_t>(max_new, some / group + 1)) : max_keys;
+    };
     const int64_t rows = (int64_t) max_new * group;
     p.chunk = rows > FEW_ROWS;
     p.few = !p.chunk || (B > 1 && group <= FEW_ROWS);
     if (p.few) {
-        // Splits up to about 16 waves per CU. Workgroups of 8 waves where they do not outnumber the CUs,
-        // of at least 2048 keys (fewer are through before a second launch has joined them), else (and
-        // beside chunks, of sequences whose number is not known) of 4 waves and 1024 keys.
         p.few_rows = (int) std::min<int64_t>(rows, FEW_ROWS);
         p.few_qt = p.few_rows <= 16 && !p.chunk ? 1 : 2;
         p.few_tiles = (p.few_rows + 16 * p.few_qt - 1) / (16 * p.few_qt);
         const int64_t pairs = (int64_t) B * n_kv;
         p.few_waves = !p.chunk && pairs * p.few_tiles <= 256 ? 8 : 4;
-        const int64_t n = std::min((4096 + p.few_waves * pairs - 1) / (p.few_waves * pairs), max_keys / (256 * p.few_waves));
+        // A workgroup alone on its CU takes 6 us and 9 us per 1000 keys of 128 (a CU's own bandwidth), so keys are
+        // split as far as the CUs go, but not below 128 keys, and only where that gains more than the second launch
+        // that joins them costs (5 us; 1 / 2 / 4 / 8 / 16 / 32 splits, us: one sequence of 8 heads of 128 over 2000
+        // keys 24 / 18 / 14 / 12 / 10 / 10, 4 over 5000 48 / 31 / 22 / 20 / 25 / 31, 16 over 4000 53 / 41 / 43 / 50 /
+        // 64 / 87, 32 over 12000 190 / 200 / 195 / 192 / 228 / 290). With more pairs than CUs workgroups have 4 waves,
+        // and are split up to about 16 waves per CU, to no less than 1024 keys (40 sequences of 8 heads of 128 over
+        // 12000 keys, 1 / 2 / 4: 269 / 227 / 216); beside chunks they have 4 waves too.
+        const int64_t keys = seen(FEW_ROWS), groups = pairs * p.few_tiles;
+        int64_t n = std::min(256 / groups, keys / 128);
+        if (n > 1 && keys * hd * (n - 1) / n <= 72 * 1024) n = 1;
+        if (!p.chunk && p.few_waves == 4) n = std::min((1024 + pairs - 1) / pairs, keys / 1024);
         p.few_split = (int) std::max<int64_t>(1, std::min<int64_t>(n, 64));
         // (chunks of max_new tokens each, unless rows are padding: no launch to join what is hardly there)
         if (p.chunk && tokens >= (int64_t) B * max_new) p.few_split = 1;
@@ -1197,7 +1218,8 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
         // row tiles of a head: at most one per CH_ROWS rows and one begun per sequence that has more than few
         const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS);
         const int64_t most = tokens * group / CH_ROWS + (p.few ? std::min<int64_t>(B, tokens * group / (FEW_ROWS + 1)) : B);
-        p.deal = deal_of(B, hd, (double) (least * n_kv), (double) p.chunk_tiles * n_kv * B, max_new, max_keys,
+        const double keys = (double) seen(CH_ROWS), mean = std::min(keys, std::max(0.0, (double) max_keys - 0.5 * max_new));
+        p.deal = deal_of(B, hd, (double) (least * n_kv), (double) p.chunk_tiles * n_kv * B, keys, mean,
                          B <= BAL_SEQS && most <= BAL_TILES);
         if (p.deal != DEAL_GRID) p.most_tiles = (int) most;
     }

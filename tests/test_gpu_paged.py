@@ -213,7 +213,8 @@ def test_strides(gpu, hd):
 
 
 @pytest.mark.parametrize("lens,nh,nkv,hd", [([(1, 5000)], 8, 1, 128), ([(1, 3001), (1, 7)], 2, 2, 32),
-                                            ([(4, 4099)], 16, 4, 64), ([(60, 5001)], 4, 2, 128)])
+                                            ([(4, 4099)], 16, 4, 64), ([(60, 5001)], 4, 2, 128),
+                                            ([(1, 3000), (2, 1801)], 64, 32, 64)])
 def test_long_sequences_split(gpu, lens, nh, nkv, hd):
     """Few rows over long sequences: the work is split over the keys and joined."""
     bt = Batch(13, lens, nh, nkv, hd, 32, "bf16")

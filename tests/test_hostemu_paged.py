@@ -47,8 +47,9 @@ def _run(check, args):
 
 
 @pytest.mark.parametrize("args", [
-    "64 1 8 2 32 0 0 1 0 0 1:5000",                          # one token: splits joined
-    "32 0 4 4 64 0 0 0 2 1 1:30000",                         # more than four of them
+    "64 1 8 2 32 0 0 1 0 0 1:5000",                          # one token: many splits joined
+    "32 0 4 4 64 0 0 0 2 1 1:30000",
+    "128 0 64 64 16 0 0 0 2 0 1:1200",                       # four splits
     "128 1 2 1 16 0 0 0 0 1 90:3000",                        # a chunk: equal runs of keys joined
     "128 0 2 1 16 0 0 0 1 2 140:2000 1:40 0:0 40:600",      # unequal row tiles beside a token
     "64 1 4 1 32 0 0 0 0 0 33:3500 40:90 1:2100",
