@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
 //   0  takes a run of key tiles: those of all row tiles in the order (head, sequence, row tile, key) are
 //      cut into equal runs, one per workgroup, and the ids of an XCD take consecutive runs. A row tile that a
 //      cut goes through is joined by k_attn_paged_join. For few row tiles over many keys.
-constexpr int BAL_GROUPS = 512, BAL_SEQS = 4096, BAL_TILES = 1536, BAL_LEAST = 4, BAL_SORT = 256;
+constexpr int BAL_GROUPS = 256, BAL_SEQS = 4096, BAL_TILES = 1536, BAL_LEAST = 4, BAL_SORT = 256;
 
 struct BalHead { int64_t run; int tiles, pad; };    // key tiles per workgroup, row tiles of a head
 struct BalTile { int first, num, b, rt; };          // a row tile's place in its head's list of key tiles
@@ -1155,23 +1155,26 @@ struct Plan {
 };
 
 // How chunks are dealt to workgroups, by estimated times in us. A step of 64 keys takes `step` with one
-// workgroup on a CU and up to twice that with two. One row tile per workgroup takes the longest row tile's
+// workgroup on a CU, and the chip as a whole `share` of that per CU with two (small heads leave one waiting
+// for its own exponentials). One row tile per workgroup takes the longest row tile's
 // steps or the chip's share of all; in the order of the grid two long ones can share a CU while the
 // chip holds about all of them (512 workgroups), by length they do not, at the price of the list. Equal
 // runs take the share and a fixed cost that grows with the partial results. `all` takes the other
 // sequences of a batch as 0.7 of the longest. Measured (us; grid order / by length / runs), heads of 128,
-// 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 233 / 224 / 246, two chunks of 700 to 1000 over 200 to
-// 4900 beside 22 single tokens 223 / 152 / 181, 3 prompts of 300 to 2500 70 / 77 / -, one of 2000 54 / 58 / 88,
-// 2 x 256 over 2900 72 / - / 52, 64 over 8000 160 / - / 40; heads of 64: 8 x 200 to 800 over up to 3800,
-// 16 over 8 - / 59 / 74, 6 x 100 to 700 over up to 3700, 32 over 8 of 128 127 / 102 / 131, a prompt of 2000, 16 over 16 35 / - / 42.
+// 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 232 / 217 / 289, two chunks of 700 to 1000 over 200 to
+// 4900 beside 22 single tokens 227 / 153 / 196, 3 prompts of 300 to 2500 74 / 82 / 185, one of 2000 54 / 59 / 140,
+// 6 x 100 to 700 over up to 3700 128 / 103 / 190, 2 x 256 over 2900 69 / 74 / 53, 64 over 8000 158 / 165 / 36;
+// 5 over 1, 4 x 100 over 7000 to 11000 beside 3 single tokens 210 / 216 / 42; heads of 64: 8 x 200 to 800 over up
+// to 3800, 16 over 8 74 / 60 / 101; heads of 32: 2 x 125 to 307 over 4600, 64 over 8 59 / 61 / 52.
 enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
 Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mean_keys, bool lists) {
-    const double step = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45, load = tiles / 256;
+    const double step = hd == 128 ? 1.0 : hd == 64 ? 0.75 : 0.7, share = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45;
+    const double load = tiles / 256;
     const double longest = keys / 64, mean = mean_keys / 64;
     // (prompts from the start come by length in the grid's order too, once there are more than fit)
     const double old = mean / std::max(longest, 1.0), shared = std::min({load - 1.0, 1.0, old > 0.7 ? 1.0 : 3.0 - load});
     const double slow = 1.1 * (1.0 + std::max(shared, 0.0) * old);
-    const double all = mean * tiles / 512 * 1.95 * step * (B > 1 ? 0.7 : 1.0);
+    const double all = mean * tiles / 512 * 1.95 * share * (B > 1 ? 0.7 : 1.0);
     // (a workgroup of the grid beyond a sequence's rows costs its start: a chunk of 4096 tokens beside 255 single
     // ones, 32 over 8 of 128, 937 us of which 0.6 ms are such workgroups; from the list 361)
     const double grid = std::max(longest * slow * step, all) + (groups - tiles) / 512;
