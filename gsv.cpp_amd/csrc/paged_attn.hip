@@ -835,7 +835,10 @@ __device__ __forceinline__ void few_beside(const PagedAttn & a, MixLds<HD> & lds
 // sequence's last, which sees the most keys, to its first: the longest workgroups start first on
 // every XCD (ids go round-robin to the 8 XCDs), and with pairs a multiple of 8 an XCD's L2 holds the
 // keys of its own pairs only (8191 tokens, 8 heads of 128: 777 us with the tiles fastest, the CUs busy
-// for 0.69 of it; 594 us so).
+// for 0.69 of it; 594 us so). An XCD deals its workgroups to 4 shader engines in turn, so the order of the
+// sequences shifts by one every second round: else an engine would get the same sequence, the longest
+// perhaps, each time (8 prompts of 700 to 4000, 16 heads over 4 of 128: 423 -> 290 us; 4 of 1428 to 3250, 64 over
+// 8: 655 -> 575; 2 of 1200 to 4000: 422 -> 374; a shift every round leaves these 2 as they were).
 template <class T, int HD>
 __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_chunk(PagedAttn a) {
     __shared__ __align__(16) MixLds<HD> lds;
@@ -844,7 +847,7 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
         return;
     }
     const int pairs = a.kv.n_kv * a.kv.B, pair = blockIdx.x % pairs;
-    const int kvh = pair % a.kv.n_kv, b = pair / a.kv.n_kv;
+    const int kvh = pair % a.kv.n_kv, b = (pair / a.kv.n_kv + (int) (blockIdx.x / pairs) / 2) % a.kv.B;
     const Seq s = seq_of(a, b);
     const int rt = (s.rows + CH_ROWS - 1) / CH_ROWS - 1 - (int) (blockIdx.x / pairs);
     if (rt < 0 || s.rows < a.min_rows) return;
@@ -1161,11 +1164,11 @@ struct Plan {
 // chip holds about all of them (512 workgroups), by length they do not, at the price of the list. Equal
 // runs take the share and a fixed cost that grows with the partial results. `all` takes the other
 // sequences of a batch as 0.7 of the longest. Measured (us; grid order / by length / runs), heads of 128,
-// 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 232 / 217 / 289, two chunks of 700 to 1000 over 200 to
-// 4900 beside 22 single tokens 227 / 153 / 196, 3 prompts of 300 to 2500 74 / 82 / 185, one of 2000 54 / 59 / 140,
-// 6 x 100 to 700 over up to 3700 128 / 103 / 190, 2 x 256 over 2900 69 / 74 / 53, 64 over 8000 158 / 165 / 36;
+// 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 237 / 220 / 289, two chunks of 700 to 1000 over 200 to
+// 4900 beside 22 single tokens 159 / 149 / 196, 3 prompts of 300 to 2500 72 / 80 / 185, one of 2000 54 / 59 / 140,
+// 6 x 100 to 700 over up to 3700 129 / 104 / 190, 2 x 256 over 2900 69 / 74 / 53, 64 over 8000 158 / 165 / 36;
 // 5 over 1, 4 x 100 over 7000 to 11000 beside 3 single tokens 210 / 216 / 42; heads of 64: 8 x 200 to 800 over up
-// to 3800, 16 over 8 74 / 60 / 101; heads of 32: 2 x 125 to 307 over 4600, 64 over 8 59 / 61 / 52.
+// to 3800, 16 over 8 70 / 59 / 101; heads of 32: 2 x 125 to 307 over 4600, 64 over 8 59 / 61 / 52.
 enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
 Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mean_keys, bool lists) {
     const double step = hd == 128 ? 1.0 : hd == 64 ? 0.75 : 0.7, share = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45;
