@@ -182,7 +182,7 @@ extern "C" int gsvk_op_paged_append(const gsvk_paged_kv * kv, const void * q, co
         a.rot = rope->rot;
         a.pairs = rope->pairs != 0;
     }
-    GSVK_REQUIRE(tokens * (nh + 2 * (int64_t) kv->n_kv) * (kv->hd / 16) <= (int64_t) INT32_MAX * AP_THREADS,
+    GSVK_REQUIRE(tokens * (nh + 2 * (int64_t) kv->n_kv) * (kv->hd / 16) <= (int64_t) UINT32_MAX - AP_THREADS,
                  "paged_append: too many elements for one launch");
     a.q = (const char *) q;
     a.k = (const char *) k;

@@ -858,7 +858,8 @@ __global__ void __launch_bounds__(CH_WAVES * 64, HD == 32 ? 4 : 2) k_attn_paged_
 // Row tiles of unequal length. Every workgroup computes the same list of row tiles and running sums of
 // their key tiles, then, by a.ordered,
 //   1  takes one whole row tile: the ids go from the longest to the shortest, so that the workgroups that share
-//      a CU, and those that come last, are not long ones by chance;
+//      a CU, and those that come last, are not long ones by chance (of more than BAL_SORT from the list's end
+//      to its start, without the sums: the count of longer ones is quadratic, and every CU gets several);
 //   0  takes a run of key tiles: those of all row tiles in the order (head, sequence, row tile, key) are
 //      cut into equal runs, one per workgroup, and the ids of an XCD take consecutive runs. A row tile that a
 //      cut goes through is joined by k_attn_paged_join. For few row tiles over many keys.
@@ -938,26 +939,27 @@ __global__ void __launch_bounds__(CH_WAVES * 64, 2) k_attn_paged_balanced(PagedA
         return;
     }
     int units = 0;   // key tiles of a head
-    for (int e0 = 0; e0 < tiles; e0 += CH_WAVES * 64) {
+    const int summed = !a.ordered || tiles <= BAL_SORT ? tiles : 0;
+    for (int e0 = 0; e0 < summed; e0 += CH_WAVES * 64) {
         int n = 0, add = 0;
         const int e = e0 + tid;
-        if (e < tiles) {
+        if (e < summed) {
             const int b = last_le(bal.tiles, a.kv.B, e);
             n = span_of(a, seq_of(a, b), e - bal.tiles[b]).num;
         }
         n = scan_group(n, bal.wave, add);
-        if (e < tiles) bal.units[e] = units + n;
+        if (e < summed) bal.units[e] = units + n;
         units += add;
     }
-    if (tid == 0) bal.units[tiles] = units;
+    if (tid == 0) bal.units[summed] = units;
     __syncthreads();
     units = __builtin_amdgcn_readfirstlane(units);
     if (a.ordered) {
         // heads fastest: an XCD keeps its heads
         const int rank = (int) blockIdx.x / a.kv.n_kv, kvh = (int) blockIdx.x % a.kv.n_kv;
         if (rank >= tiles) return;
-        int e = rank;
-        if (tiles <= BAL_SORT) {   // (the count is quadratic, and of more every CU gets several)
+        int e = tiles - 1 - rank;
+        if (tiles <= BAL_SORT) {
             if (tid < tiles) {
                 const int n = bal.units[tid + 1] - bal.units[tid];
                 int r = 0;
@@ -1162,7 +1164,7 @@ struct Plan {
 // for its own exponentials). One row tile per workgroup takes the longest row tile's
 // steps or the chip's share of all; in the order of the grid two long ones can share a CU while the
 // chip holds about all of them (512 workgroups), by length they do not, at the price of the list. Equal
-// runs take the share and a fixed cost that grows with the partial results. `all` takes the other
+// runs, one workgroup on a CU, take 1.4 of the share and a fixed cost that grows with the partial results. `all` takes the other
 // sequences of a batch as 0.7 of the longest. Measured (us; grid order / by length / runs), heads of 128,
 // 32 over 8: 4 x 512 tokens over 1000 to 8100 keys 237 / 220 / 289, two chunks of 700 to 1000 over 200 to
 // 4900 beside 22 single tokens 159 / 149 / 196, 3 prompts of 300 to 2500 72 / 80 / 185, one of 2000 54 / 59 / 140,
@@ -1170,7 +1172,7 @@ struct Plan {
 // 5 over 1, 4 x 100 over 7000 to 11000 beside 3 single tokens 210 / 216 / 42; heads of 64: 8 x 200 to 800 over up
 // to 3800, 16 over 8 70 / 59 / 101; heads of 32: 2 x 125 to 307 over 4600, 64 over 8 59 / 61 / 52.
 enum Deal { DEAL_GRID, DEAL_LENGTH, DEAL_RUNS };
-Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mean_keys, bool lists) {
+Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mean_keys, int64_t most) {
     const double step = hd == 128 ? 1.0 : hd == 64 ? 0.75 : 0.7, share = hd == 128 ? 1.0 : hd == 64 ? 0.6 : 0.45;
     const double load = tiles / 256;
     const double longest = keys / 64, mean = mean_keys / 64;
@@ -1181,9 +1183,12 @@ Deal deal_of(int B, int hd, double tiles, double groups, double keys, double mea
     // (a workgroup of the grid beyond a sequence's rows costs its start: a chunk of 4096 tokens beside 255 single
     // ones, 32 over 8 of 128, 937 us of which 0.6 ms are such workgroups; from the list 361)
     const double grid = std::max(longest * slow * step, all) + (groups - tiles) / 512;
-    const double length = B > 1 ? std::max(1.1 * longest * step, all) + 6 + B / 512.0 : 1e30;   // (one sequence's go well as they are)
-    const double runs = all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
-    if (!lists || grid <= std::min(length, runs)) return DEAL_GRID;
+    // (one sequence's go well as they are; not put in order the list's end is worse than the grid's, 605 to 575)
+    double length = std::max(1.1 * longest * step, most > BAL_SORT ? 1.1 * all : all) + 6 + B / 512.0;
+    if (B == 1 || B > BAL_SEQS || most > UINT16_MAX) length = 1e30;
+    double runs = 1.4 * all + 22 + 30 * std::min(1.0, tiles / 512) * hd / 128;
+    if (B > BAL_SEQS || most > BAL_TILES) runs = 1e30;
+    if (grid <= std::min(length, runs)) return DEAL_GRID;
     return length <= runs ? DEAL_LENGTH : DEAL_RUNS;
 }
 
@@ -1225,8 +1230,7 @@ Plan plan_of(int B, int n_kv, int hd, int group, int64_t tokens, int max_new, in
         const int64_t least = std::max<int64_t>(1, tokens * group / CH_ROWS);
         const int64_t most = tokens * group / CH_ROWS + (p.few ? std::min<int64_t>(B, tokens * group / (FEW_ROWS + 1)) : B);
         const double keys = (double) seen(CH_ROWS), mean = std::min(keys, std::max(0.0, (double) max_keys - 0.5 * max_new));
-        p.deal = deal_of(B, hd, (double) (least * n_kv), (double) p.chunk_tiles * n_kv * B, keys, mean,
-                         B <= BAL_SEQS && most <= BAL_TILES);
+        p.deal = deal_of(B, hd, (double) (least * n_kv), (double) p.chunk_tiles * n_kv * B, keys, mean, most);
         if (p.deal != DEAL_GRID) p.most_tiles = (int) most;
     }
     return p;
@@ -1347,7 +1351,9 @@ extern "C" int gsvk_op_attn_paged(const gsvk_paged_kv * kv, const void * q, int6
     const size_t need = space_of(p, tokens * nh, kv->n_kv, kv->hd).end;
     GSVK_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t) ws & 15) == 0),
                  "attn_paged: a workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", need, ws_bytes);
-    GSVK_REQUIRE(groups_of(p, kv->B, kv->n_kv) <= INT32_MAX && join_groups_of(p, kv->B, kv->n_kv, kv->hd) <= INT32_MAX,
+    // (a launch has fewer than 2^32 threads)
+    constexpr int64_t MOST = UINT32_MAX / 256;
+    GSVK_REQUIRE(groups_of(p, kv->B, kv->n_kv) <= MOST && join_groups_of(p, kv->B, kv->n_kv, kv->hd) <= MOST,
                  "attn_paged: too many row tiles for one launch");
     a.q = (const uint16_t *) q;
     a.q_stride = q_stride;

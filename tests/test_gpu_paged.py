@@ -306,6 +306,14 @@ def test_chunks_among_many_sequences(gpu, chunks, window):
     _attn(gpu, Batch(21, lens, 8, 1, 32, 16, "f16", tail=1), window=window)
 
 
+def test_more_row_tiles_than_are_summed(gpu):
+    """More row tiles of a head than a workgroup has sums for (wide groups), taken whole from the list."""
+    lens = [(1, 1 + b % 50) for b in range(300)]
+    for i in range(6):
+        lens[40 * i + 3] = (1100 + 10 * i, 1200)
+    _attn(gpu, Batch(22, lens, 32, 1, 32, 16, "bf16", tail=1))
+
+
 def test_nothing_to_do(gpu):
     """No rows, no sequences, sequences without rows: nothing is written and nothing fails."""
     bt = Batch(18, [(0, 20), (0, 0)], 4, 2, 64, 16, "f16", tail=4)

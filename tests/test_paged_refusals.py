@@ -88,6 +88,14 @@ def _ws(kv, tokens, nh, max_new, max_keys):
     return gsvk.lib().gsvk_attn_paged_workspace_bytes(C.byref(kv), tokens, nh, max_new, max_keys, 0)
 
 
+def test_more_work_than_a_launch_holds_is_refused():
+    """2^32 threads or more: said before the launch."""
+    assert _append(_kv(n_kv=16, hd=128), tokens=2 ** 25, nh=64, qs=8192, ks=2048, vs=2048) == 1
+    assert "too many" in gsvk.last_error()
+    assert _attn(_kv(n_kv=8, hd=64, B=65535), tokens=2 ** 24, nh=64, qs=4096, os_=4096, max_new=8192, max_keys=8192) == 1
+    assert "too many" in gsvk.last_error()
+
+
 def test_workspace_is_asked_for():
     """One long sequence is split over its keys: a call without the workspace it needs is refused; one
     short sequence needs none."""
